@@ -1,0 +1,214 @@
+// Products on grouped rows: what the kernels of experts (ep_grouped.hip) and of low-rank adapters (ep_low_rank.hip) share.
+//
+// Rows p = offsets[g] .. offsets[g + 1] - 1 of the grouped order meet the weight of group g; places from offsets[groups] on
+// belong to no group. The sizes of the groups are known on the device only, so a launch covers the most row tiles there can
+// be (every group may end inside a tile) and a block finds its tile by a scan over the offsets.
+#pragma once
+
+#include "ep_matrix.hpp"
+
+namespace ep {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int64_t kMostEntries = int64_t{1} << 30;
+
+struct RowTile {
+  int group;       // `groups` for a tile of rows without a group, -1 past the last tile
+  int first;       // first place of the tile
+  int rows;        // 1 .. tile_rows places
+  int index;       // number of the tile within its group
+};
+
+// Tile number `tile` of tiles of `tile_rows` places, in the order of the groups, those of no group last. Called by whole
+// waves; the result is the same in every lane.
+__device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ offsets, int groups, int entries, int tile, int tile_rows) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int g0 = 0; g0 < groups; g0 += 64) {
+    const int g = g0 + lane;
+    int low = 0, high = 0;
+    if (g < groups) {
+      low = offsets[g];
+      high = offsets[g + 1];
+    }
+    const int n = (high - low + tile_rows - 1) / tile_rows;
+    int inclusive = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int other = __shfl_up(inclusive, d);
+      if (lane >= d) inclusive += other;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + inclusive > tile);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      const int index = tile - before - __builtin_amdgcn_readlane(inclusive - n, at);
+      const int first = __builtin_amdgcn_readlane(low, at) + index * tile_rows;
+      const int left = __builtin_amdgcn_readlane(high, at) - first;
+      return {g0 + at, first, left < tile_rows ? left : tile_rows, index};
+    }
+    before += __builtin_amdgcn_readlane(inclusive, 63);
+  }
+  const int kept = __builtin_amdgcn_readfirstlane(offsets[groups]);
+  const int64_t first = kept + static_cast<int64_t>(tile - before) * tile_rows;
+  if (first >= entries) return {-1, 0, 0, 0};
+  const int64_t left = entries - first;
+  return {groups, static_cast<int>(first), static_cast<int>(left < tile_rows ? left : tile_rows), tile - before};
+}
+
+// The most tiles of `tile_rows` places that `entries` places in `groups` groups (and the places of none) make.
+inline int64_t most_row_tiles(int64_t entries, int groups, int tile_rows) {
+  const int64_t parts = groups + 1 < entries ? groups + 1 : entries;          // every part may end with a tile of its own
+  return entries / tile_rows + parts;
+}
+
+// What a product on grouped rows is told. Row p reads row order[p] / per_row of x, or row p where order is null.
+struct GroupedArgs {
+  const uint8_t* x;
+  const uint8_t* w;
+  const float* scale_x;            // int8 products: per row of x, per row of every weight
+  const float* scale_w;
+  const void* bias;                // [groups][N], in the output's type
+  void* y;
+  const int32_t* order;
+  const int32_t* offsets;
+  int64_t ldx_bytes, ldw_bytes, group_bytes, k_bytes, ldy;
+  int entries, groups, N, per_row, x_rows, out_kind;
+};
+
+__device__ __forceinline__ int source_row(const GroupedArgs& a, int place) {
+  if (a.order == nullptr) return place;
+  const int row = static_cast<int>(static_cast<uint32_t>(a.order[place]) / static_cast<uint32_t>(a.per_row));
+  return row < a.x_rows ? row : a.x_rows - 1;
+}
+
+// ---- few rows per group: the weight's stream bounds the product -------------------------------------------------------------
+//
+// A block takes 16 MT rows and 16 NT weight rows; its waves take every WAVES-th piece of 256 bytes of K and the sums meet in
+// LDS. Both operands go from memory straight into the fragments of the 16 x 16 matrix-core instructions (lane l holds 16
+// bytes of row l % 16 at byte 16 (l / 16) of a 64-byte step: 64 consecutive bytes per row and instruction), so there is no
+// barrier in the loop and every wave keeps 4 (MT + NT) loads of 1 KiB in flight.
+// PLANES: the sums are multiplied with scale_x[group] and stored as two bf16 parts, the rounded value and the rounded
+// remainder, columns [0, padded) and [padded, 2 padded) of row p of y, padded = N rounded up to 16; columns from N on are 0.
+// The product that reads them then works on 16 bits of significand instead of 8, in the memory that f32 would take.
+template <bool INT8, int MT, int NT, int WAVES, bool PLANES>
+__global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs a) {
+  using Acc = typename std::conditional<INT8, i32x4, f32x4>::type;
+  using Frag = typename std::conditional<INT8, i32x4, bf16x8>::type;
+  using Cell = typename std::conditional<INT8, int32_t, float>::type;
+  constexpr int kRows = 16 * MT, kColumns = 16 * NT, kPitch = kColumns + 4;
+  __shared__ __align__(16) Cell sums[WAVES][kRows][kPitch];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int column_tiles = (a.N + kColumns - 1) / kColumns;
+  const int n0 = static_cast<int>(blockIdx.x % column_tiles) * kColumns;
+  const RowTile tile = find_row_tile(a.offsets, a.groups, a.entries, static_cast<int>(blockIdx.x / column_tiles), kRows);
+  if (tile.group < 0) return;
+  if (tile.group == a.groups) {
+    if constexpr (!PLANES) {                       // rows of no group
+      for (int cell = threadIdx.x; cell < kRows * kColumns; cell += 64 * WAVES) {
+        const int row = cell / kColumns, n = n0 + cell % kColumns;
+        if (row < tile.rows && n < a.N) store_out(a.y, a.out_kind, (static_cast<int64_t>(tile.first) + row) * a.ldy + n, 0.0f);
+      }
+    }
+    return;
+  }
+  const int in_row = lane & 15, piece = (lane >> 4) * 16;
+  const uint8_t* from_x[MT];
+  const uint8_t* from_w[NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int row = 16 * t + in_row;
+    from_x[t] = a.x + source_row(a, tile.first + (row < tile.rows ? row : tile.rows - 1)) * a.ldx_bytes + piece;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = n0 + 16 * j + in_row;
+    from_w[j] = a.w + tile.group * a.group_bytes + (n < a.N ? n : a.N - 1) * a.ldw_bytes + piece;
+  }
+  Acc acc[MT][NT] = {};
+  auto multiply = [&](const uint4 (&fx)[MT], const uint4 (&fw)[NT]) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (INT8) acc[t][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(Frag, fx[t]), __builtin_bit_cast(Frag, fw[j]), acc[t][j], 0, 0, 0);
+        else acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Frag, fx[t]), __builtin_bit_cast(Frag, fw[j]), acc[t][j], 0, 0, 0);
+      }
+  };
+  int64_t kb = wave * 256;
+  for (; kb + 256 <= a.k_bytes; kb += WAVES * 256) {
+    uint4 fx[4][MT], fw[4][NT];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fw[s][j] = *reinterpret_cast<const uint4*>(from_w[j] + kb + 64 * s);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) fx[s][t] = *reinterpret_cast<const uint4*>(from_x[t] + kb + 64 * s);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) multiply(fx[s], fw[s]);
+  }
+  if (kb < a.k_bytes) {                            // the last, partial piece: both operands are zero past the row's end
+#pragma unroll 1
+    for (int s = 0; s < 4; ++s) {
+      uint4 fx[MT], fw[NT];
+      const bool inside = kb + 64 * s + piece < a.k_bytes;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) fx[t] = inside ? *reinterpret_cast<const uint4*>(from_x[t] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fw[j] = inside ? *reinterpret_cast<const uint4*>(from_w[j] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
+      multiply(fx, fw);
+    }
+  }
+  // Register i of lane l holds row 4 (l / 16) + i and column l % 16 of its 16 x 16 tile.
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[wave][16 * t + 4 * (lane >> 4) + i][16 * j + in_row] = acc[t][j][i];
+  __syncthreads();
+  for (int cell = threadIdx.x; cell < kRows * kColumns; cell += 64 * WAVES) {
+    const int row = cell / kColumns, column = cell % kColumns, n = n0 + column;
+    if (row >= tile.rows) continue;
+    Cell sum = sums[0][row][column];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) sum += sums[w][row][column];
+    const int64_t place = static_cast<int64_t>(tile.first) + row;
+    if constexpr (PLANES) {
+      const int padded = (a.N + 15) & ~15;
+      if (n >= padded) continue;
+      float v = n < a.N ? static_cast<float>(sum) : 0.0f;
+      if (a.scale_x != nullptr && n < a.N) v *= a.scale_x[tile.group];
+      uint16_t* out = static_cast<uint16_t*>(a.y) + place * a.ldy + n;
+      const uint32_t high = bf16_bits_of(v);
+      const float rest = v - __uint_as_float(high << 16);
+      out[0] = static_cast<uint16_t>(high);
+      out[padded] = (high & 0x7F80u) == 0x7F80u ? 0 : static_cast<uint16_t>(bf16_bits_of(rest));    // an infinity has no remainder
+    } else if (n < a.N) {
+      const bool has_bias = a.bias != nullptr;
+      const float b = has_bias ? load_bias(a.bias, a.out_kind, tile.group * a.N + n) : 0.0f;
+      float v;
+      if constexpr (INT8) {
+        // int32 -> f32, times the activation row's scale, times the weight row's, plus bias: each one rounded operation.
+        v = __fmul_rn(__fmul_rn(static_cast<float>(sum), a.scale_x[source_row(a, tile.first + row)]), a.scale_w[static_cast<int64_t>(tile.group) * a.N + n]);
+        if (has_bias) v = __fadd_rn(v, b);
+      } else {
+        v = static_cast<float>(sum) + b;
+      }
+      store_out(a.y, a.out_kind, place * a.ldy + n, v);
+    }
+  }
+}
+
+template <bool INT8, int MT, int NT, int WAVES, bool PLANES>
+static int launch_stream_of(const GroupedArgs& a, hipStream_t s) {
+  const int64_t blocks = most_row_tiles(a.entries, a.groups, 16 * MT) * ((a.N + 16 * NT - 1) / (16 * NT));
+  if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+  hipLaunchKernelGGL((grouped_stream_kernel<INT8, MT, NT, WAVES, PLANES>), dim3(static_cast<unsigned>(blocks)), dim3(64 * WAVES), 0, s, a);
+  EP_HIP_TRY(hipGetLastError());
+  return EP_HIP_OK;
+}
+
+}  // namespace ep

@@ -1,0 +1,183 @@
+"""Low-rank adapters of many requests beside a shared, compressed projection.
+
+`low_rank_update(y, x, down, up, groups, scale)` adds to the shared projection's output y each row's own update,
+scale[a] * (x down[a]^T) up[a]^T, for rows that name their adapter (`group_rows(ids, adapters)`, made once per step and used
+by every layer). `AdaptedLinear` wraps a compressed layer with a bank of adapters; the compressed weight stays frozen, the
+adapters train. The reference has no counterpart.
+"""
+from __future__ import annotations
+
+import torch
+
+from ..backends import hip as _hip
+from .groups import RowGroups, device_of, matrix
+from .linear import CompressedLinear
+
+
+def _shrink(x, down, scale, groups: RowGroups) -> torch.Tensor:
+    """scale[a] * x down[a]^T per place, as two bf16 parts (value, remainder) of `rank` rounded up to 16 columns each."""
+    rank = down.shape[1]
+    planes = torch.empty(groups.entries, 2 * (-(-rank // 16) * 16), dtype=torch.bfloat16, device=x.device)
+    rows, narrow = matrix(x, 8), matrix(down, 8)
+    with torch.cuda.device(x.device):
+        _hip.check("ep_hip_low_rank_shrink", _hip.library().ep_hip_low_rank_shrink(
+            rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0), None if scale is None else scale.data_ptr(),
+            planes.data_ptr(), groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, rows.shape[1],
+            _hip.current_stream(x.device)))
+    return planes
+
+
+def _expand(planes, up, y, groups: RowGroups) -> torch.Tensor:
+    """y + planes up[a]^T, rows of no group as they are in y (zero where y is None)."""
+    outer, rank = up.shape[1], up.shape[2]
+    out = torch.empty(groups.entries, outer, dtype=torch.bfloat16, device=planes.device)
+    if y is not None and not (y.stride(1) == 1 and y.stride(0) >= outer):
+        y = y.contiguous()
+    with torch.cuda.device(planes.device):
+        _hip.check("ep_hip_low_rank_expand", _hip.library().ep_hip_low_rank_expand(
+            planes.data_ptr(), up.data_ptr(), up.stride(1), up.stride(0), None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
+            out.data_ptr(), outer, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, outer,
+            _hip.current_stream(planes.device)))
+    return out
+
+
+def _reduce(planes, rank: int, rows, transposed: bool, groups: RowGroups) -> torch.Tensor:
+    """Per adapter the sum over its places of planes^T rows: [adapters, rank, width], or [adapters, width, rank] transposed."""
+    width = rows.shape[1]
+    rows = matrix(rows, 8)
+    out = torch.empty((groups.groups, width, rank) if transposed else (groups.groups, rank, width), dtype=torch.bfloat16, device=planes.device)
+    with torch.cuda.device(planes.device):
+        _hip.check("ep_hip_low_rank_reduce", _hip.library().ep_hip_low_rank_reduce(
+            planes.data_ptr(), rows.data_ptr(), rows.stride(0), out.data_ptr(), int(transposed), groups.order.data_ptr(), groups.offsets.data_ptr(),
+            groups.entries, groups.groups, rank, width, _hip.current_stream(planes.device)))
+    return out
+
+
+class _LowRankUpdate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, down, up, scale, groups):
+        planes = _shrink(x.detach(), down.detach(), scale, groups)
+        out = _expand(planes, up.detach().contiguous(), y.detach(), groups)
+        ctx.groups = groups
+        ctx.save_for_backward(x, down, up, scale, planes if ctx.needs_input_grad[3] else None)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, down, up, scale, planes = ctx.saved_tensors
+        groups, (need_y, need_x, need_down, need_up) = ctx.groups, ctx.needs_input_grad[:4]
+        grad_x = grad_down = grad_up = None
+        if need_x or need_down:
+            # The gradient of the narrow rows is a shrink by up^T, that of x an expand by down^T: two small transposes.
+            narrow = _shrink(grad, up.transpose(1, 2).contiguous(), scale, groups)
+            if need_x:
+                grad_x = _expand(narrow, down.transpose(1, 2).contiguous(), None, groups)
+            if need_down:
+                grad_down = _reduce(narrow, down.shape[1], x, False, groups)
+        if need_up:
+            grad_up = _reduce(planes, up.shape[2], grad, True, groups)
+        return grad if need_y else None, grad_x, grad_down, grad_up, None, None
+
+
+def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, groups: RowGroups,
+                    scale: torch.Tensor | None = None) -> torch.Tensor:
+    """y[t] + scale[a] * (x[t] @ down[a].T) @ up[a].T with a = the adapter of row t; rows without one come back as y.
+
+    Args:
+        y: bf16 [tokens, out_features], the shared projection's output.
+        x: bf16 [tokens, in_features], its input.
+        down: bf16 [adapters, rank, in_features]. up: bf16 [adapters, out_features, rank].
+        groups: the plan of `group_rows(ids, adapters)` with one id per token.
+        scale: f32 [adapters] or None for ones; it gets no gradient.
+
+    Sums are f32; the narrow rows between the two products are kept in 16 bits of significand; the result is rounded to
+    bf16 once. Differentiable in y, x, down and up.
+    """
+    if not isinstance(groups, RowGroups):
+        raise TypeError(f"low_rank_update takes the plan that group_rows returns, got {type(groups).__name__}")
+    for name, tensor in (("y", y), ("x", x), ("down", down), ("up", up)):
+        if tensor.dtype != torch.bfloat16:
+            raise TypeError(f"low_rank_update takes bfloat16 operands, got {name} in {tensor.dtype}")
+    if groups.per_row != 1:
+        raise ValueError(f"low_rank_update takes one adapter per row, the plan has {groups.per_row}")
+    if down.dim() != 3 or up.dim() != 3 or down.shape[0] != groups.groups or up.shape[0] != groups.groups or down.shape[1] != up.shape[2]:
+        raise ValueError(f"low_rank_update takes down [{groups.groups}, rank, in_features] and up [{groups.groups}, out_features, rank], "
+                         f"got {tuple(down.shape)} and {tuple(up.shape)}")
+    if tuple(x.shape) != (groups.tokens, down.shape[2]) or tuple(y.shape) != (groups.tokens, up.shape[1]):
+        raise ValueError(f"low_rank_update takes x of shape {(groups.tokens, down.shape[2])} and y of shape {(groups.tokens, up.shape[1])}, "
+                         f"got {tuple(x.shape)} and {tuple(y.shape)}")
+    if 0 in down.shape or 0 in up.shape:
+        raise ValueError("low_rank_update needs at least one feature and rank one")
+    if down.shape[1] > 4096:
+        raise ValueError(f"low_rank_update takes ranks up to 4096, got {down.shape[1]}")
+    if scale is not None:
+        if tuple(scale.shape) != (groups.groups,):
+            raise ValueError(f"low_rank_update takes one scale per adapter, got shape {tuple(scale.shape)}")
+        if scale.requires_grad:
+            raise ValueError("low_rank_update gives no gradient of the scale: detach it")
+        scale = scale.float().contiguous()
+    device_of("low_rank_update", y, x, down, up, groups.order, scale)
+    if groups.tokens == 0:
+        return y + (x.sum() + down.sum() + up.sum()) * 0
+    return _LowRankUpdate.apply(y, x, down, up, scale, groups)
+
+
+class AdaptedLinear(torch.nn.Module):
+    """A compressed linear layer with a bank of low-rank adapters, one of them (or none) per activation row.
+
+    Args:
+        base: a `CompressedLinear` or a subclass of it; its weight stays frozen.
+        adapters: how many the bank holds. rank: of every adapter; a smaller one is stored padded with zeros.
+
+    `down` starts with small random values and `up` with zeros, so that a new adapter changes nothing until it is trained or set;
+    both are trainable parameters. `scale` is a buffer of ones.
+    """
+
+    def __init__(self, base: CompressedLinear, adapters: int, rank: int):
+        super().__init__()
+        if not isinstance(base, CompressedLinear):
+            raise TypeError(f"AdaptedLinear takes a compressed linear layer, got {type(base).__name__}")
+        for name, value in (("adapters", adapters), ("rank", rank)):
+            if isinstance(value, bool) or not isinstance(value, int) or value < 1:
+                raise ValueError(f"{name} must be a positive integer, got {value!r}")
+        self.base = base
+        device = base.device
+        self.down = torch.nn.Parameter(torch.randn(adapters, rank, base.in_features, device=device).mul_(base.in_features ** -0.5).bfloat16())
+        self.up = torch.nn.Parameter(torch.zeros(adapters, base.out_features, rank, dtype=torch.bfloat16, device=device))
+        self.register_buffer("scale", torch.ones(adapters, device=device))
+
+    @property
+    def adapters(self) -> int:
+        return self.down.shape[0]
+
+    @property
+    def rank(self) -> int:
+        return self.down.shape[1]
+
+    @torch.no_grad()
+    def set_adapter(self, index: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:
+        """Stores one adapter: down [r, in_features], up [out_features, r], r at most the bank's rank."""
+        if not 0 <= index < self.adapters:
+            raise IndexError(f"adapter {index} of a bank of {self.adapters}")
+        rank = down.shape[0]
+        if rank > self.rank or tuple(down.shape) != (rank, self.base.in_features) or tuple(up.shape) != (self.base.out_features, rank):
+            raise ValueError(f"an adapter of this bank has down [r, {self.base.in_features}] and up [{self.base.out_features}, r] with r up to "
+                             f"{self.rank}, got {tuple(down.shape)} and {tuple(up.shape)}")
+        self.down[index].zero_()
+        self.up[index].zero_()
+        self.down[index, :rank].copy_(down)
+        self.up[index, :, :rank].copy_(up)
+        self.scale[index] = scale
+
+    def forward(self, x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
+        """base(x) plus every row's update; x [.., in_features] in bf16, `groups` one id per row of x."""
+        y = self.base(x)
+        rows = low_rank_update(y.reshape(-1, y.shape[-1]), x.reshape(-1, x.shape[-1]), self.down, self.up, groups, self.scale)
+        return rows.reshape(y.shape)
+
+    def extra_repr(self) -> str:
+        return f"adapters={self.adapters}, rank={self.rank}"
+
+
+__all__ = ["AdaptedLinear", "low_rank_update"]

@@ -1,0 +1,200 @@
+"""Rows grouped by an id: the plan that products by expert and adapters by request share, and the weighted return.
+
+`group_rows(ids, groups)` sorts the entries of `ids` (one per token, or k per token) by group on the device and returns a
+`RowGroups`; `linear.grouped` multiplies each group with its own weight, `linear.adapters` adds each group's low-rank
+update, and `combine_rows` brings grouped rows back to their tokens. Sizes of groups stay on the device: nothing here
+synchronises, and every call may be captured into a graph (the ids may then change between replays). The reference has no
+counterpart: its layers have one weight each (entropack/linear/linear.py:18-230).
+
+Capturing a training step: run forward and backward inside the same capture, and let no eager graph over the same leaves
+live meanwhile (torch ties a leaf's gradient accumulation to the stream it was first used on).
+"""
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+from ..backends import hip as _hip
+
+MAX_GROUPS = 896                   # a thread per group and 64 KiB of LDS in the sorting kernel
+MAX_ENTRIES = 1 << 30
+_ROW_KINDS = {torch.bfloat16: 0, torch.float32: 2}
+
+
+def device_of(name: str, *tensors: torch.Tensor | None) -> torch.device:
+    """The one GPU all operands are on."""
+    device = None
+    for tensor in tensors:
+        if tensor is None:
+            continue
+        if tensor.device.type != "cuda":
+            raise RuntimeError(f"{name} runs on the GPU, got a tensor on {tensor.device}")
+        if device is None:
+            device = tensor.device
+        elif tensor.device != device:
+            raise ValueError(f"{name}: all operands must be on one device, got {device} and {tensor.device}")
+    return device
+
+
+def matrix(tensor: torch.Tensor, pieces: int) -> torch.Tensor:
+    """`tensor` ([.., columns]) as the kernels read it: columns contiguous, rows and groups whole numbers of 16 bytes apart and
+    not overlapping, the first row 16-byte aligned. Rows of a number of columns that is no multiple of `pieces` are padded
+    with zeros. A tensor that lies so already is returned as it is; anything else is copied."""
+    columns = tensor.shape[-1]
+    if columns % pieces:
+        return torch.nn.functional.pad(tensor, (0, pieces - columns % pieces))
+    fits = tensor.stride(-1) == 1 and tensor.data_ptr() % 16 == 0
+    least = columns
+    for dim in range(tensor.dim() - 2, -1, -1):
+        fits = fits and tensor.stride(dim) >= least and tensor.stride(dim) % pieces == 0
+        least = tensor.stride(dim) * (tensor.shape[dim] - 1) + least
+    return tensor if fits else tensor.clone(memory_format=torch.contiguous_format)
+
+
+@dataclasses.dataclass(frozen=True, eq=False)
+class RowGroups:
+    """What `group_rows` made of a tensor of ids. Made by `group_rows` only: the kernels take its indices as they are.
+
+    Attributes:
+        order: int32 [entries], the entries (token * per_row + pick) sorted by group, those of no group last.
+        offsets: int32 [groups + 1], the first place of every group; places from offsets[groups] on have no group.
+        place: int32 [entries], the inverse of `order`.
+        groups: number of groups.
+        tokens, per_row: the ids' shape; entries = tokens * per_row.
+    """
+    order: torch.Tensor
+    offsets: torch.Tensor
+    place: torch.Tensor
+    groups: int
+    tokens: int
+    per_row: int
+
+    @property
+    def entries(self) -> int:
+        return self.tokens * self.per_row
+
+    @property
+    def device(self) -> torch.device:
+        return self.order.device
+
+
+def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
+    """Sorts the entries of `ids` (int32 or int64, [tokens] or [tokens, k], on the GPU) by group.
+
+    Ids outside [0, groups), such as -1 for padding, belong to no group: the products give those rows zero (the adapters
+    leave them as they are), the weighted return skips them. The sort is stable, so the result is the same in every run.
+    """
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"group_rows takes int32 or int64 ids, got {ids.dtype}")
+    if ids.dim() not in (1, 2):
+        raise ValueError(f"group_rows takes ids of shape [tokens] or [tokens, k], got {tuple(ids.shape)}")
+    if isinstance(groups, bool) or not isinstance(groups, int) or not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"groups must be an integer from 1 to {MAX_GROUPS}, got {groups!r}")
+    tokens, per_row = ids.shape[0], 1 if ids.dim() == 1 else ids.shape[1]
+    if per_row < 1:
+        raise ValueError("group_rows needs at least one id per token")
+    entries = tokens * per_row
+    if entries > MAX_ENTRIES:
+        raise ValueError(f"group_rows takes at most {MAX_ENTRIES} entries, got {entries}")
+    device = device_of("group_rows", ids)
+    order = torch.empty(entries, dtype=torch.int32, device=device)
+    place = torch.empty(entries, dtype=torch.int32, device=device)
+    if entries == 0:
+        return RowGroups(order, torch.zeros(groups + 1, dtype=torch.int32, device=device), place, groups, tokens, per_row)
+    offsets = torch.empty(groups + 1, dtype=torch.int32, device=device)
+    flat = ids.contiguous()
+    with torch.cuda.device(device):
+        lib = _hip.library()
+        room = lib.ep_hip_group_rows_workspace(entries, groups)
+        workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+        _hip.check("ep_hip_group_rows", lib.ep_hip_group_rows(
+            flat.data_ptr(), flat.element_size(), entries, groups, order.data_ptr(), offsets.data_ptr(), place.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), room, _hip.current_stream(device)))
+    return RowGroups(order, offsets, place, groups, tokens, per_row)
+
+
+def kept_rows(groups: RowGroups) -> int:
+    """Address of the number of places that have a group."""
+    return groups.offsets.data_ptr() + 4 * groups.groups
+
+
+def sum_entries(rows: torch.Tensor, tokens: int, per_row: int) -> torch.Tensor:
+    """[entries, width] rows in the order of the entries (f32 or bf16) added up per token, rounded to bf16 once."""
+    out = torch.empty(tokens, rows.shape[1], dtype=torch.bfloat16, device=rows.device)
+    if out.numel():
+        with torch.cuda.device(rows.device):
+            _hip.check("ep_hip_combine_rows", _hip.library().ep_hip_combine_rows(
+                rows.data_ptr(), _ROW_KINDS[rows.dtype], rows.stride(0), None, None, None, 0, per_row, tokens, rows.shape[1],
+                out.data_ptr(), out.stride(0), _hip.current_stream(rows.device)))
+    return out
+
+
+def _rows_of(tensor: torch.Tensor) -> torch.Tensor:
+    """Rows at any address the element-wise kernels take: columns contiguous, rows not overlapping."""
+    return tensor if tensor.stride(1) == 1 and tensor.stride(0) >= tensor.shape[1] else tensor.contiguous()
+
+
+class _CombineRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weight, groups):
+        rows = _rows_of(y.detach())
+        ready = None if weight is None else weight.detach().contiguous()
+        out = torch.empty(groups.tokens, y.shape[1], dtype=torch.bfloat16, device=y.device)
+        if out.numel():
+            with torch.cuda.device(y.device):
+                _hip.check("ep_hip_combine_rows", _hip.library().ep_hip_combine_rows(
+                    rows.data_ptr(), _ROW_KINDS[torch.bfloat16], rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
+                    None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
+                    groups.tokens, rows.shape[1], out.data_ptr(), out.stride(0), _hip.current_stream(y.device)))
+        ctx.groups = groups
+        ctx.save_for_backward(y, weight)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weight = ctx.saved_tensors
+        groups, (need_y, need_weight, _) = ctx.groups, ctx.needs_input_grad
+        grad_y = torch.empty_like(y, memory_format=torch.contiguous_format) if need_y else None
+        grad_weight = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_weight else None
+        if y.numel():
+            rows, ready, slope = _rows_of(y), None if weight is None else weight.contiguous(), _rows_of(grad)
+            with torch.cuda.device(y.device):
+                _hip.check("ep_hip_combine_rows_grad", _hip.library().ep_hip_combine_rows_grad(
+                    slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
+                    None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
+                    groups.tokens, rows.shape[1], None if grad_y is None else grad_y.data_ptr(), rows.shape[1],
+                    None if grad_weight is None else grad_weight.data_ptr(), _hip.current_stream(y.device)))
+        elif grad_weight is not None:
+            grad_weight.zero_()
+        return grad_y, grad_weight, None
+
+
+def combine_rows(y: torch.Tensor, groups: RowGroups, weight: torch.Tensor | None = None) -> torch.Tensor:
+    """Grouped rows back to their tokens: out[t] = sum over t's entries of weight[t, j] * y[place of the entry].
+
+    Args:
+        y: bf16 [entries, width] in grouped order, as `grouped_linear` returns it.
+        groups: the plan of `group_rows`.
+        weight: f32 or bf16, the shape of the ids, or None for ones (the router's weights).
+
+    Entries of no group add nothing, whatever y and weight hold there. Sums are f32, rounded to bf16 once. Differentiable
+    in y and weight.
+    """
+    if not isinstance(groups, RowGroups):
+        raise TypeError(f"combine_rows takes the plan that group_rows returns, got {type(groups).__name__}")
+    if y.dtype != torch.bfloat16:
+        raise TypeError(f"combine_rows takes bfloat16 rows, got {y.dtype}")
+    if y.dim() != 2 or y.shape[0] != groups.entries:
+        raise ValueError(f"combine_rows takes {groups.entries} rows (one per entry), got shape {tuple(y.shape)}")
+    if weight is not None:
+        if weight.dtype not in _ROW_KINDS:
+            raise TypeError(f"combine_rows takes float32 or bfloat16 weights, got {weight.dtype}")
+        if tuple(weight.shape) not in ({(groups.tokens, groups.per_row)} | ({(groups.tokens,)} if groups.per_row == 1 else set())):
+            raise ValueError(f"combine_rows takes weights of shape {(groups.tokens, groups.per_row)}, got {tuple(weight.shape)}")
+    device_of("combine_rows", y, groups.order, weight)
+    return _CombineRows.apply(y, weight, groups)
+
+
+__all__ = ["RowGroups", "combine_rows", "group_rows"]
