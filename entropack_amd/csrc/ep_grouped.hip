@@ -1,8 +1,8 @@
 // Products of grouped rows with the weight of their group (a mixture's experts), and their gradients.
 //
-//   y[p]  = x[order[p] / k] . w[g]^T (+ bias[g])            few rows per group: grouped_stream_kernel (ep_grouped.hpp), else grouped_tile_kernel
+//   y[p]  = x[rows[p]] . w[g]^T (+ bias[g])            few rows per group: grouped_stream_kernel (ep_grouped.hpp), else grouped_tile_kernel
 //   dx[p] = dy[p] . w[g]                                    grouped_tile_kernel (ep_grouped_tile.hpp)
-//   dw[g] = sum_p dy[p]^T x[order[p] / k]                   grouped_tile_kernel
+//   dw[g] = sum_p dy[p]^T x[rows[p]]                        grouped_tile_kernel
 //   db[g] = sum_p dy[p]                                     grouped_column_sums_kernel
 #include "ep_grouped_tile.hpp"
 
@@ -29,10 +29,9 @@ __global__ __launch_bounds__(256) void grouped_column_sums_kernel(const uint16_t
 
 // ---- checks that every entry point makes --------------------------------------------------------------------------------------
 
-static bool groups_valid(const int32_t* offsets, int64_t entries, int groups, const int32_t* order, int per_row, int64_t x_rows) {
+static bool groups_valid(const int32_t* offsets, int64_t entries, int groups, const int32_t* row_of, int64_t x_rows) {
   if (offsets == nullptr || entries <= 0 || groups <= 0 || entries > kMostEntries) return false;
-  if (order != nullptr) return per_row >= 1 && x_rows >= 1 && x_rows <= 0x7FFFFFFF;
-  return x_rows >= entries;
+  return row_of != nullptr ? x_rows >= 1 && x_rows <= 0x7FFFFFFF : x_rows >= entries && x_rows <= 0x7FFFFFFF;
 }
 
 static bool kind_valid(int kind) { return kind == kOutBF16 || kind == kOutF16 || kind == kOutF32; }
@@ -46,11 +45,20 @@ static bool rows_in_pieces(const void* base, int64_t ld, int64_t K, int element_
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld >= K && (ld * element_bytes) % 16 == 0 && (K * element_bytes) % 16 == 0;
 }
 
-template <bool INT8, int MODE>
+template <bool INT8, int MODE, bool GATHER = true>
 static int launch_tile(const TileArgs& t, int64_t row_tiles, hipStream_t s) {
   const int64_t blocks = row_tiles * ((t.columns + kTile - 1) / kTile);
   if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
-  hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, t);
+  const bool whole = MODE == kForward ? t.inner % 128 == 0 : (MODE == kGradRows && t.inner % 128 == 0 && t.columns % kTile == 0);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if constexpr (MODE != kGradWeight) {
+    if (whole) {
+      hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, false, GATHER>), grid, dim3(256), 0, s, t);
+      EP_HIP_TRY(hipGetLastError());
+      return EP_HIP_OK;
+    }
+  }
+  hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, true, GATHER>), grid, dim3(256), 0, s, t);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
 }
@@ -59,9 +67,9 @@ template <bool INT8>
 static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
   if (a.entries / a.groups < 32) return launch_stream_of<INT8, 1, 2, 4, false>(a, s);
   TileArgs t = {};
-  t.a = a.x, t.b = a.w, t.scale_x = a.scale_x, t.scale_w = a.scale_w, t.bias = a.bias, t.y = a.y, t.order = a.order, t.offsets = a.offsets;
+  t.a = a.x, t.b = a.w, t.scale_x = a.scale_x, t.scale_w = a.scale_w, t.bias = a.bias, t.y = a.y, t.row_of = a.row_of, t.offsets = a.offsets;
   t.lda_bytes = a.ldx_bytes, t.ldb_bytes = a.ldw_bytes, t.group_b_bytes = a.group_bytes, t.ldy = a.ldy;
-  t.entries = a.entries, t.groups = a.groups, t.per_row = a.per_row, t.x_rows = a.x_rows, t.out_kind = a.out_kind;
+  t.entries = a.entries, t.groups = a.groups, t.x_rows = a.x_rows, t.out_kind = a.out_kind;
   t.columns = a.N, t.inner = static_cast<int>(a.k_bytes);
   return launch_tile<INT8, kForward>(t, most_row_tiles(a.entries, a.groups, kTile), s);
 }
@@ -71,62 +79,64 @@ static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
 extern "C" {
 
 int ep_hip_grouped_gemm_bf16(const void* x_dev, int64_t ldx, int64_t x_rows, const void* w_dev, int64_t ldw, int64_t w_group, const void* bias_dev, void* y_dev,
-                             int64_t ldy, int out_kind, const int32_t* order_dev, int per_row, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
+                             int64_t ldy, int out_kind, const int32_t* rows_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
                              int64_t K, void* stream) {
   using namespace ep;
-  if (x_dev == nullptr || w_dev == nullptr || y_dev == nullptr || !groups_valid(offsets_dev, entries, groups, order_dev, per_row, x_rows)) return EP_HIP_EINVAL;
+  if (x_dev == nullptr || w_dev == nullptr || y_dev == nullptr || !groups_valid(offsets_dev, entries, groups, rows_dev, x_rows)) return EP_HIP_EINVAL;
   if (!sizes_valid(N, K, groups) || !kind_valid(out_kind) || ldy < N) return EP_HIP_EINVAL;
   if (!rows_in_pieces(x_dev, ldx, K, 2) || !rows_in_pieces(w_dev, ldw, K, 2) || w_group % 8 != 0 || w_group < 0) return EP_HIP_EINVAL;
   GroupedArgs a = {};
-  a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(w_dev), a.bias = bias_dev, a.y = y_dev, a.order = order_dev, a.offsets = offsets_dev;
+  a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(w_dev), a.bias = bias_dev, a.y = y_dev, a.row_of = rows_dev, a.offsets = offsets_dev;
   a.ldx_bytes = ldx * 2, a.ldw_bytes = ldw * 2, a.group_bytes = w_group * 2, a.k_bytes = K * 2, a.ldy = ldy;
-  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(N), a.per_row = per_row, a.x_rows = static_cast<int>(x_rows), a.out_kind = out_kind;
+  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(N), a.x_rows = static_cast<int>(x_rows), a.out_kind = out_kind;
   return launch_grouped<false>(a, static_cast<hipStream_t>(stream));
 }
 
 int ep_hip_grouped_gemm_i8(const int8_t* x_dev, int64_t ldx, int64_t x_rows, const int8_t* w_dev, int64_t ldw, int64_t w_group, const float* scale_x_dev,
-                           const float* scale_w_dev, const void* bias_dev, void* y_dev, int64_t ldy, int out_kind, const int32_t* order_dev, int per_row,
+                           const float* scale_w_dev, const void* bias_dev, void* y_dev, int64_t ldy, int out_kind, const int32_t* rows_dev,
                            const int32_t* offsets_dev, int64_t entries, int groups, int64_t N, int64_t K, void* stream) {
   using namespace ep;
   if (x_dev == nullptr || w_dev == nullptr || y_dev == nullptr || scale_x_dev == nullptr || scale_w_dev == nullptr) return EP_HIP_EINVAL;
-  if (!groups_valid(offsets_dev, entries, groups, order_dev, per_row, x_rows)) return EP_HIP_EINVAL;
+  if (!groups_valid(offsets_dev, entries, groups, rows_dev, x_rows)) return EP_HIP_EINVAL;
   if (!sizes_valid(N, K, groups) || !kind_valid(out_kind) || ldy < N) return EP_HIP_EINVAL;
   if (!rows_in_pieces(x_dev, ldx, K, 1) || !rows_in_pieces(w_dev, ldw, K, 1) || w_group % 16 != 0 || w_group < 0) return EP_HIP_EINVAL;
   GroupedArgs a = {};
   a.x = reinterpret_cast<const uint8_t*>(x_dev), a.w = reinterpret_cast<const uint8_t*>(w_dev), a.scale_x = scale_x_dev, a.scale_w = scale_w_dev;
-  a.bias = bias_dev, a.y = y_dev, a.order = order_dev, a.offsets = offsets_dev;
+  a.bias = bias_dev, a.y = y_dev, a.row_of = rows_dev, a.offsets = offsets_dev;
   a.ldx_bytes = ldx, a.ldw_bytes = ldw, a.group_bytes = w_group, a.k_bytes = K, a.ldy = ldy;
-  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(N), a.per_row = per_row, a.x_rows = static_cast<int>(x_rows), a.out_kind = out_kind;
+  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(N), a.x_rows = static_cast<int>(x_rows), a.out_kind = out_kind;
   return launch_grouped<true>(a, static_cast<hipStream_t>(stream));
 }
 
 int ep_hip_grouped_grad_rows_bf16(const void* dy_dev, int64_t lddy, const void* w_dev, int64_t ldw, int64_t w_group, void* dx_dev, int64_t lddx, int out_kind,
                                   const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N, int64_t K, void* stream) {
   using namespace ep;
-  if (dy_dev == nullptr || w_dev == nullptr || dx_dev == nullptr || !groups_valid(offsets_dev, entries, groups, order_dev, 1, entries)) return EP_HIP_EINVAL;
+  if (dy_dev == nullptr || w_dev == nullptr || dx_dev == nullptr || !groups_valid(offsets_dev, entries, groups, order_dev, entries)) return EP_HIP_EINVAL;
   if (!sizes_valid(N, K, groups) || !kind_valid(out_kind) || lddx < K) return EP_HIP_EINVAL;
   if (!rows_in_pieces(dy_dev, lddy, (N + 7) / 8 * 8, 2) || !rows_in_pieces(w_dev, ldw, K, 2) || w_group % 8 != 0 || w_group < 0) return EP_HIP_EINVAL;
   TileArgs t = {};
   t.a = static_cast<const uint8_t*>(dy_dev), t.b = static_cast<const uint8_t*>(w_dev), t.y = dx_dev, t.order = order_dev, t.offsets = offsets_dev;
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldw * 2, t.group_b_bytes = w_group * 2, t.ldy = lddx;
-  t.entries = static_cast<int>(entries), t.groups = groups, t.per_row = 1, t.x_rows = static_cast<int>(entries), t.out_kind = out_kind;
+  t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(entries), t.out_kind = out_kind;
   t.columns = static_cast<int>(K), t.inner = static_cast<int>(N * 2);
   return launch_tile<false, kGradRows>(t, most_row_tiles(entries, groups, kTile), static_cast<hipStream_t>(stream));
 }
 
 int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void* x_dev, int64_t ldx, int64_t x_rows, void* dw_dev, int64_t lddw, int64_t dw_group,
-                                    int out_kind, const int32_t* order_dev, int per_row, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
+                                    int out_kind, const int32_t* rows_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
                                     int64_t K, void* stream) {
   using namespace ep;
-  if (dy_dev == nullptr || x_dev == nullptr || dw_dev == nullptr || !groups_valid(offsets_dev, entries, groups, order_dev, per_row, x_rows)) return EP_HIP_EINVAL;
+  if (dy_dev == nullptr || x_dev == nullptr || dw_dev == nullptr || !groups_valid(offsets_dev, entries, groups, rows_dev, x_rows)) return EP_HIP_EINVAL;
   if (!sizes_valid(N, K, groups) || !kind_valid(out_kind) || lddw < K || dw_group < 0) return EP_HIP_EINVAL;
   if (!rows_in_pieces(dy_dev, lddy, N, 2) || !rows_in_pieces(x_dev, ldx, K, 2)) return EP_HIP_EINVAL;
   TileArgs t = {};
-  t.a = static_cast<const uint8_t*>(dy_dev), t.b = static_cast<const uint8_t*>(x_dev), t.y = dw_dev, t.order = order_dev, t.offsets = offsets_dev;
+  t.a = static_cast<const uint8_t*>(dy_dev), t.b = static_cast<const uint8_t*>(x_dev), t.y = dw_dev, t.row_of = rows_dev, t.offsets = offsets_dev;
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldx * 2, t.ldy = lddw, t.group_y = dw_group;
-  t.entries = static_cast<int>(entries), t.groups = groups, t.per_row = per_row, t.x_rows = static_cast<int>(x_rows), t.out_kind = out_kind;
+  t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(x_rows), t.out_kind = out_kind;
   t.rows = static_cast<int>(N), t.columns = static_cast<int>(K);
-  return launch_tile<false, kGradWeight>(t, static_cast<int64_t>(groups) * ((N + kTile - 1) / kTile), static_cast<hipStream_t>(stream));
+  const int64_t row_tiles = static_cast<int64_t>(groups) * ((N + kTile - 1) / kTile);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return rows_dev != nullptr ? launch_tile<false, kGradWeight, true>(t, row_tiles, s) : launch_tile<false, kGradWeight, false>(t, row_tiles, s);
 }
 
 int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int32_t* offsets_dev, int groups, int64_t N, void* out_dev, int out_kind, void* stream) {

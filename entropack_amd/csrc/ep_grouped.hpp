@@ -62,7 +62,7 @@ inline int64_t most_row_tiles(int64_t entries, int groups, int tile_rows) {
   return entries / tile_rows + parts;
 }
 
-// What a product on grouped rows is told. Row p reads row order[p] / per_row of x, or row p where order is null.
+// What a product on grouped rows is told. Place p reads row row_of[p] of x, or row p where row_of is null.
 struct GroupedArgs {
   const uint8_t* x;
   const uint8_t* w;
@@ -70,15 +70,15 @@ struct GroupedArgs {
   const float* scale_w;
   const void* bias;                // [groups][N], in the output's type
   void* y;
-  const int32_t* order;
+  const int32_t* row_of;
   const int32_t* offsets;
   int64_t ldx_bytes, ldw_bytes, group_bytes, k_bytes, ldy;
-  int entries, groups, N, per_row, x_rows, out_kind;
+  int entries, groups, N, x_rows, out_kind;
 };
 
 __device__ __forceinline__ int source_row(const GroupedArgs& a, int place) {
-  if (a.order == nullptr) return place;
-  const int row = static_cast<int>(static_cast<uint32_t>(a.order[place]) / static_cast<uint32_t>(a.per_row));
+  if (a.row_of == nullptr) return place;
+  const int row = a.row_of[place];
   return row < a.x_rows ? row : a.x_rows - 1;
 }
 

@@ -31,10 +31,11 @@ struct TileArgs {
   const float* scale_w;
   const void* bias;                // forward: [groups][columns], in the output's type
   void* y;
-  const int32_t* order;            // forward: rows of a are read at order[p] / per_row; weights' gradient: rows of b are; rows' gradient:
-  const int32_t* offsets;          //   rows of y are written at order[p]
+  const int32_t* row_of;           // forward: place p reads row row_of[p] of a; weights' gradient: of b (null: row p)
+  const int32_t* order;            // rows' gradient: place p is written to row order[p] of y (null: row p)
+  const int32_t* offsets;
   int64_t lda_bytes, ldb_bytes, group_b_bytes, ldy, group_y;
-  int entries, groups, per_row, x_rows, out_kind;
+  int entries, groups, x_rows, out_kind;
   int rows;                        // weights' gradient: rows of y (columns of a)
   int columns;                     // columns of y
   int inner;                       // forward, rows' gradient: the inner length in bytes of the row operand
@@ -44,7 +45,10 @@ enum : int { kForward = 0, kGradRows = 1, kGradWeight = 2 };
 
 constexpr int kTile = 128, kTileStage = 2 * 128 * 128;      // a stage: 16 KiB of each operand
 
-template <bool INT8, int MODE>
+// TAIL = false: the inner length is a whole number of steps (and, in the rows' gradient, the columns a whole number of tiles), so
+// that no piece lies outside.
+// GATHER: the weights' gradient with row_of (the other modes look at the pointer).
+template <bool INT8, int MODE, bool TAIL, bool GATHER>
 __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(TileArgs g) {
   static_assert(!INT8 || MODE == kForward, "gradients are bf16");
   constexpr bool kColumnA = MODE == kGradWeight, kColumnB = MODE != kForward;
@@ -80,8 +84,8 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(TileArgs g) {
   const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeroPiece);
 
   auto source_of = [&](int place) {
-    if (g.order == nullptr) return place;
-    const int row = static_cast<int>(static_cast<uint32_t>(g.order[place]) / static_cast<uint32_t>(g.per_row));
+    if (g.row_of == nullptr) return place;
+    const int row = g.row_of[place];
     return row < g.x_rows ? row : g.x_rows - 1;
   };
 
@@ -118,35 +122,35 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(TileArgs g) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int at = 64 * step + 4 * (wave + 4 * c) + (lane >> 4);
-        row_b[c] = source_of(first + (at < inner ? at : inner - 1));
+        const int place = first + (at < inner ? at : inner - 1);
+        row_b[c] = GATHER ? g.row_of[place] : place;
       }
     }
   };
   auto to_lds = [&](const uint8_t* from, uint8_t* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
   };
+  auto select = [&](bool inside, const uint8_t* from) {     // bitwise: a branch here would break the flow of the K loop
+    const uint64_t mask = inside ? ~uint64_t{0} : 0;
+    return reinterpret_cast<const uint8_t*>((reinterpret_cast<uint64_t>(from) & mask) | (reinterpret_cast<uint64_t>(zeros) & ~mask));
+  };
   auto load_a = [&](uint8_t* stage, int step, int c) {
     const uint8_t* from;
-    if constexpr (kColumnA) {
-      from = from_a[c] + step * (64 * g.lda_bytes);
-      if (a_outside || 64 * step + 4 * (wave + 4 * c) + (lane >> 4) >= inner) from = zeros;
-    } else {
-      from = from_a[c] + step * int64_t{128};
-      if (128 * step + 16 * piece_r >= inner) from = zeros;
-    }
+    if constexpr (kColumnA) from = select(!a_outside & (64 * step + 4 * (wave + 4 * c) + (lane >> 4) < inner), from_a[c] + step * (64 * g.lda_bytes));
+    else if constexpr (TAIL) from = select(128 * step + 16 * piece_r < inner, from_a[c] + step * int64_t{128});
+    else from = from_a[c] + step * int64_t{128};
     to_lds(from, stage + 1024 * (wave + 4 * c));
   };
   auto load_b = [&](uint8_t* stage, int step, int c) {
     const uint8_t* from;
     if constexpr (MODE == kForward) {
-      from = from_b[c] + step * int64_t{128};
-      if (128 * step + 16 * piece_r >= inner) from = zeros;
+      if constexpr (TAIL) from = select(128 * step + 16 * piece_r < inner, from_b[c] + step * int64_t{128});
+      else from = from_b[c] + step * int64_t{128};
     } else if constexpr (MODE == kGradRows) {
-      from = from_b[c] + step * (64 * g.ldb_bytes);
-      if (b_outside || 2 * (64 * step + 4 * (wave + 4 * c) + (lane >> 4)) >= inner) from = zeros;
+      if constexpr (TAIL) from = select(!b_outside & (2 * (64 * step + 4 * (wave + 4 * c) + (lane >> 4)) < inner), from_b[c] + step * (64 * g.ldb_bytes));
+      else from = from_b[c] + step * (64 * g.ldb_bytes);
     } else {
-      from = from_b[c] + row_b[c] * g.ldb_bytes;
-      if (b_outside || 64 * step + 4 * (wave + 4 * c) + (lane >> 4) >= inner) from = zeros;
+      from = select(!b_outside & (64 * step + 4 * (wave + 4 * c) + (lane >> 4) < inner), from_b[c] + (row_b[c] < g.x_rows ? row_b[c] : g.x_rows - 1) * g.ldb_bytes);
     }
     to_lds(from, stage + 16384 + 1024 * (wave + 4 * c));
   };
@@ -238,10 +242,12 @@ __global__ __launch_bounds__(256, 2) void grouped_tile_kernel(TileArgs g) {
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 4; ++t) read_one(0, stage0, 0, t);
-    for (int step = 0; step < steps; step += 2) {
+    int step = 0;
+    for (; step + 2 <= steps; step += 2) {                  // (a branch between the two steps would cost a wait for all loads)
       k_step(stage0, stage1, step);
-      if (step + 1 < steps) k_step(stage1, stage0, step + 1);
+      k_step(stage1, stage0, step + 1);
     }
+    if (step < steps) k_step(stage0, stage1, step);
     __builtin_amdgcn_s_waitcnt(0x0F70);
   }
   __syncthreads();                                          // every load has landed and every fragment is read: the stages are free

@@ -1,7 +1,7 @@
 // Entries grouped by an id, and the weighted return of grouped rows to their tokens.
 //
-//   group_rows_*      a stable counting sort of small integers: order (entries sorted by id, "no group" last), offsets (first
-//                     place of every group) and place (the inverse of order). Integer work only; the result does not depend
+//   group_*           a stable counting sort of small integers: order (entries sorted by id, "no group" last), offsets (first
+//                     place of every group), place (the inverse of order), rows (order / per_row). Integer work only; the result does not depend
 //                     on timing: a wave counts 64 consecutive entries at a time by comparing their ids with ballots, bit by
 //                     bit, so that an entry's rank among equal ids is a population count.
 //   combine_*         out[t] = sum_j w[t, j] y[place[t k + j]] and its gradients. Bound by the rows of y.
@@ -45,7 +45,7 @@ __device__ __forceinline__ void count_entries(const Id* __restrict__ ids, int64_
 // Gives every entry its place; next[key] (LDS, this wave's row) is the place of the wave's next entry with that key.
 template <typename Id>
 __device__ __forceinline__ void place_entries(const Id* __restrict__ ids, int64_t first, int64_t last, int groups, int key_bits, int* next,
-                                              int32_t* __restrict__ order, int32_t* __restrict__ place) {
+                                              int per_row, int32_t* __restrict__ order, int32_t* __restrict__ place, int32_t* __restrict__ rows) {
   const int lane = threadIdx.x & 63;
   for (int64_t at = first; at < last; at += 64) {
     const bool live = at + lane < last;
@@ -56,6 +56,7 @@ __device__ __forceinline__ void place_entries(const Id* __restrict__ ids, int64_
       const int to = base + __builtin_popcountll(same & ((uint64_t{1} << lane) - 1));
       order[to] = static_cast<int32_t>(at + lane);
       place[at + lane] = to;
+      if (rows != nullptr) rows[to] = static_cast<int32_t>(static_cast<uint32_t>(at + lane) / static_cast<uint32_t>(per_row));
       __builtin_amdgcn_wave_barrier();           // the leader moves the row on once every lane of the wave has read it
       if (__builtin_ctzll(same) == lane) next[key] = base + __builtin_popcountll(same);
     }
@@ -89,9 +90,9 @@ __global__ __launch_bounds__(kGroupThreads) void group_count_kernel(const Id* __
 // LDS: per-wave rows [kGroupWaves][keys], then before[keys] (entries of a key in earlier blocks) and total[keys].
 template <typename Id>
 __global__ __launch_bounds__(kGroupThreads) void group_place_kernel(const Id* __restrict__ ids, int64_t entries, int64_t chunk, int groups,
-                                                                    int key_bits, const int32_t* __restrict__ table, int blocks,
+                                                                    int key_bits, const int32_t* __restrict__ table, int blocks, int per_row,
                                                                     int32_t* __restrict__ order, int32_t* __restrict__ offsets,
-                                                                    int32_t* __restrict__ place) {
+                                                                    int32_t* __restrict__ place, int32_t* __restrict__ rows) {
   extern __shared__ int group_smem[];
   __shared__ int wave_sums[kGroupWaves];
   const int keys = groups + 1;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_place_kernel(const Id* __
     }
   }
   __syncthreads();
-  place_entries(ids, first, last, groups, key_bits, group_smem + wave * keys, order, place);
+  place_entries(ids, first, last, groups, key_bits, group_smem + wave * keys, per_row, order, place, rows);
 }
 
 // Entries one block sorts before another block takes the rest, and the most blocks.
@@ -162,7 +163,8 @@ static int64_t group_chunk(int64_t entries) {
 }
 
 template <typename Id>
-static int launch_group(const Id* ids, int64_t entries, int groups, int32_t* order, int32_t* offsets, int32_t* place, int32_t* table, hipStream_t s) {
+static int launch_group(const Id* ids, int64_t entries, int groups, int per_row, int32_t* order, int32_t* offsets, int32_t* place, int32_t* rows, int32_t* table,
+                        hipStream_t s) {
   const int64_t chunk = group_chunk(entries);
   const int blocks = static_cast<int>((entries + chunk - 1) / chunk);
   const int keys = groups + 1;
@@ -173,7 +175,7 @@ static int launch_group(const Id* ids, int64_t entries, int groups, int32_t* ord
     EP_HIP_TRY(hipGetLastError());
   }
   hipLaunchKernelGGL(group_place_kernel<Id>, dim3(blocks), dim3(kGroupThreads), (kGroupWaves + 2) * keys * sizeof(int), s, ids, entries, chunk, groups, key_bits,
-                     blocks > 1 ? table : nullptr, blocks, order, offsets, place);
+                     blocks > 1 ? table : nullptr, blocks, per_row, order, offsets, place, rows);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
 }
@@ -312,18 +314,18 @@ size_t ep_hip_group_rows_workspace(int64_t entries, int groups) {
   return blocks > 1 ? static_cast<size_t>(blocks) * static_cast<size_t>(groups + 1) * 4 : 0;
 }
 
-int ep_hip_group_rows(const void* ids_dev, int id_bytes, int64_t entries, int groups, int32_t* order_dev, int32_t* offsets_dev, int32_t* place_dev,
-                      void* workspace_dev, size_t workspace_bytes, void* stream) {
+int ep_hip_group_rows(const void* ids_dev, int id_bytes, int64_t entries, int groups, int per_row, int32_t* order_dev, int32_t* offsets_dev, int32_t* place_dev,
+                      int32_t* rows_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
   using namespace ep;
   if (ids_dev == nullptr || order_dev == nullptr || offsets_dev == nullptr || place_dev == nullptr) return EP_HIP_EINVAL;
-  if (entries <= 0 || groups <= 0 || (id_bytes != 4 && id_bytes != 8)) return EP_HIP_EINVAL;
+  if (entries <= 0 || groups <= 0 || per_row <= 0 || (id_bytes != 4 && id_bytes != 8)) return EP_HIP_EINVAL;
   if (entries > kMostEntries || groups > kMostGroups) return EP_HIP_EUNSUPPORTED;
   const size_t wanted = ep_hip_group_rows_workspace(entries, groups);
   if (wanted != 0 && (workspace_dev == nullptr || workspace_bytes < wanted)) return EP_HIP_EINVAL;
   int32_t* table = static_cast<int32_t*>(workspace_dev);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (id_bytes == 4) return launch_group(static_cast<const int32_t*>(ids_dev), entries, groups, order_dev, offsets_dev, place_dev, table, s);
-  return launch_group(static_cast<const int64_t*>(ids_dev), entries, groups, order_dev, offsets_dev, place_dev, table, s);
+  if (id_bytes == 4) return launch_group(static_cast<const int32_t*>(ids_dev), entries, groups, per_row, order_dev, offsets_dev, place_dev, rows_dev, table, s);
+  return launch_group(static_cast<const int64_t*>(ids_dev), entries, groups, per_row, order_dev, offsets_dev, place_dev, rows_dev, table, s);
 }
 
 int ep_hip_combine_rows(const void* y_dev, int y_kind, int64_t ldy, const int32_t* place_dev, const int32_t* kept_rows_dev, const void* weight_dev, int weight_kind,

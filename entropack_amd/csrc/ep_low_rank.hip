@@ -166,9 +166,9 @@ int ep_hip_low_rank_shrink(const void* x_dev, int64_t ldx, const void* down_dev,
   if (K % 8 != 0 || ldx % 8 != 0 || ldd % 8 != 0 || down_group % 8 != 0 || ldx < K || ldd < K || down_group < 0) return EP_HIP_EINVAL;
   if (reinterpret_cast<uintptr_t>(x_dev) % 16 != 0 || reinterpret_cast<uintptr_t>(down_dev) % 16 != 0 || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
   GroupedArgs a = {};
-  a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(down_dev), a.scale_x = scale_dev, a.y = planes_dev, a.order = order_dev, a.offsets = offsets_dev;
+  a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(down_dev), a.scale_x = scale_dev, a.y = planes_dev, a.row_of = order_dev, a.offsets = offsets_dev;
   a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = (rank + 15) / 16 * 16 * 2;
-  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(rank), a.per_row = 1, a.x_rows = static_cast<int>(entries), a.out_kind = kOutBF16;
+  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(entries), a.out_kind = kOutBF16;
   return launch_stream_of<false, 1, 1, 4, true>(a, static_cast<hipStream_t>(stream));
 }
 

@@ -45,7 +45,7 @@ def _forward(x, weight, bias, groups: RowGroups, x_grouped: bool) -> torch.Tenso
             _hip.check("ep_hip_grouped_gemm_bf16", _hip.library().ep_hip_grouped_gemm_bf16(
                 rows.data_ptr(), rows.stride(0), rows.shape[0], w.data_ptr(), w.stride(1), w.stride(0),
                 None if ready is None else ready.data_ptr(), y.data_ptr(), outer, _hip.FLOAT_KINDS[torch.bfloat16],
-                None if x_grouped else groups.order.data_ptr(), groups.per_row, groups.offsets.data_ptr(), groups.entries,
+                None if x_grouped else groups.rows.data_ptr(), groups.offsets.data_ptr(), groups.entries,
                 groups.groups, outer, rows.shape[1], _hip.current_stream(x.device)))
     return y
 
@@ -79,7 +79,7 @@ def _grad_weight(grad, x, weight, groups: RowGroups, x_grouped: bool) -> torch.T
     with torch.cuda.device(grad.device):
         _hip.check("ep_hip_grouped_grad_weight_bf16", _hip.library().ep_hip_grouped_grad_weight_bf16(
             dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), rows.shape[0], out.data_ptr(), inner, outer * inner,
-            _hip.FLOAT_KINDS[torch.bfloat16], None if x_grouped else groups.order.data_ptr(), groups.per_row,
+            _hip.FLOAT_KINDS[torch.bfloat16], None if x_grouped else groups.rows.data_ptr(),
             groups.offsets.data_ptr(), groups.entries, groups.groups, outer, inner, _hip.current_stream(grad.device)))
     return out if tuple(out.shape) == tuple(weight.shape) else out[:, :weight.shape[1], :weight.shape[2]].contiguous()
 
@@ -167,7 +167,7 @@ def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups
         _hip.check("ep_hip_grouped_gemm_i8", _hip.library().ep_hip_grouped_gemm_i8(
             rows.data_ptr(), rows.stride(0), rows.shape[0], w.data_ptr(), w.stride(1), w.stride(0), scale_x.data_ptr(), scale_w.data_ptr(),
             None if ready is None else ready.data_ptr(), y.data_ptr(), outer, _hip.FLOAT_KINDS[out_dtype],
-            None if x_grouped else groups.order.data_ptr(), groups.per_row, groups.offsets.data_ptr(), groups.entries, groups.groups,
+            None if x_grouped else groups.rows.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups,
             outer, rows.shape[1], _hip.current_stream(device)))
     return y
 

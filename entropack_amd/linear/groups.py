@@ -60,12 +60,14 @@ class RowGroups:
         order: int32 [entries], the entries (token * per_row + pick) sorted by group, those of no group last.
         offsets: int32 [groups + 1], the first place of every group; places from offsets[groups] on have no group.
         place: int32 [entries], the inverse of `order`.
+        rows: int32 [entries], the token of every place (`order` itself for one id per token).
         groups: number of groups.
         tokens, per_row: the ids' shape; entries = tokens * per_row.
     """
     order: torch.Tensor
     offsets: torch.Tensor
     place: torch.Tensor
+    rows: torch.Tensor
     groups: int
     tokens: int
     per_row: int
@@ -100,8 +102,9 @@ def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
     device = device_of("group_rows", ids)
     order = torch.empty(entries, dtype=torch.int32, device=device)
     place = torch.empty(entries, dtype=torch.int32, device=device)
+    rows = torch.empty(entries, dtype=torch.int32, device=device) if per_row > 1 else order
     if entries == 0:
-        return RowGroups(order, torch.zeros(groups + 1, dtype=torch.int32, device=device), place, groups, tokens, per_row)
+        return RowGroups(order, torch.zeros(groups + 1, dtype=torch.int32, device=device), place, rows, groups, tokens, per_row)
     offsets = torch.empty(groups + 1, dtype=torch.int32, device=device)
     flat = ids.contiguous()
     with torch.cuda.device(device):
@@ -109,9 +112,9 @@ def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
         room = lib.ep_hip_group_rows_workspace(entries, groups)
         workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         _hip.check("ep_hip_group_rows", lib.ep_hip_group_rows(
-            flat.data_ptr(), flat.element_size(), entries, groups, order.data_ptr(), offsets.data_ptr(), place.data_ptr(),
-            None if workspace is None else workspace.data_ptr(), room, _hip.current_stream(device)))
-    return RowGroups(order, offsets, place, groups, tokens, per_row)
+            flat.data_ptr(), flat.element_size(), entries, groups, per_row, order.data_ptr(), offsets.data_ptr(), place.data_ptr(),
+            rows.data_ptr() if per_row > 1 else None, None if workspace is None else workspace.data_ptr(), room, _hip.current_stream(device)))
+    return RowGroups(order, offsets, place, rows, groups, tokens, per_row)
 
 
 def kept_rows(groups: RowGroups) -> int:

@@ -418,13 +418,14 @@ int ep_hip_tile_ans_encode(const uint8_t* bytes_dev, int64_t num_elements, int n
  * Not in the reference, whose layers have one weight each. An entry is one (token, pick) pair, entry = token * per_row + pick;
  * its id names its group, an id outside [0, groups) no group. `order` lists the entries sorted by group (entries of one group in
  * their own order, those of no group last), `offsets` (int32[groups + 1]) the first place of every group in that list,
- * `place` is the inverse of `order`. Rows "in grouped order" lie one per place. The products below take order, offsets and
- * place as ep_hip_group_rows wrote them. At most 2^30 entries and 896 groups. */
+ * `place` is the inverse of `order`. Rows "in grouped order" lie one per place. The products below take order, offsets,
+ * place and rows as ep_hip_group_rows wrote them. At most 2^30 entries and 896 groups. */
 
-/* ids_dev: int32 or int64 (id_bytes 4 or 8) [entries]; order_dev, place_dev: int32[entries]; offsets_dev: int32[groups + 1].
+/* ids_dev: int32 or int64 (id_bytes 4 or 8) [entries]; order_dev, place_dev: int32[entries]; offsets_dev: int32[groups + 1];
+ * rows_dev (int32[entries], NULL when not wanted): the token of every place, order / per_row.
  * workspace_dev: ep_hip_group_rows_workspace(entries, groups) bytes (0 for small calls: then it may be NULL). */
-int ep_hip_group_rows(const void* ids_dev, int id_bytes, int64_t entries, int groups, int32_t* order_dev, int32_t* offsets_dev, int32_t* place_dev,
-                      void* workspace_dev, size_t workspace_bytes, void* stream);
+int ep_hip_group_rows(const void* ids_dev, int id_bytes, int64_t entries, int groups, int per_row, int32_t* order_dev, int32_t* offsets_dev, int32_t* place_dev,
+                      int32_t* rows_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 size_t ep_hip_group_rows_workspace(int64_t entries, int groups);
 
 /* out[t] (bf16, ldo elements apart) = sum over j < per_row of weight[t][j] * y[place[t * per_row + j]], f32 sums in the order of j,
@@ -438,26 +439,26 @@ int ep_hip_combine_rows_grad(const void* grad_dev, int64_t ldg, const void* y_de
                              const void* weight_dev, int weight_kind, int per_row, int64_t tokens, int64_t width, void* grad_y_dev, int64_t ldgy,
                              void* grad_weight_dev, void* stream);
 
-/* y[p] (grouped order, ldy elements apart, out_kind 0 bf16, 1 f16, 2 f32) = x[order[p] / per_row] . w[g]^T + bias[g] for the places p of
+/* y[p] (grouped order, ldy elements apart, out_kind 0 bf16, 1 f16, 2 f32) = x[rows[p]] . w[g]^T + bias[g] for the places p of
  * group g, zero for places of no group. w: [groups][N][K], rows ldw and groups w_group elements apart; bias: [groups][N] in the
- * output's type, may be NULL. order_dev NULL: x lies in grouped order (x_rows >= entries). K in whole pieces of 16 bytes (a
+ * output's type, may be NULL. rows_dev NULL: x lies in grouped order (x_rows >= entries). K in whole pieces of 16 bytes (a
  * multiple of 8 bf16, 16 int8), x and w 16-byte aligned with row strides of whole pieces. The int8 product sums in int32 and
  * rounds f32(sum) * scale_x[row of x] * scale_w[g][n] + bias operation by operation, as ep_hip_gemm_i8 does. */
 int ep_hip_grouped_gemm_bf16(const void* x_dev, int64_t ldx, int64_t x_rows, const void* w_dev, int64_t ldw, int64_t w_group, const void* bias_dev, void* y_dev,
-                             int64_t ldy, int out_kind, const int32_t* order_dev, int per_row, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
+                             int64_t ldy, int out_kind, const int32_t* rows_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
                              int64_t K, void* stream);
 int ep_hip_grouped_gemm_i8(const int8_t* x_dev, int64_t ldx, int64_t x_rows, const int8_t* w_dev, int64_t ldw, int64_t w_group, const float* scale_x_dev,
-                           const float* scale_w_dev, const void* bias_dev, void* y_dev, int64_t ldy, int out_kind, const int32_t* order_dev, int per_row,
+                           const float* scale_w_dev, const void* bias_dev, void* y_dev, int64_t ldy, int out_kind, const int32_t* rows_dev,
                            const int32_t* offsets_dev, int64_t entries, int groups, int64_t N, int64_t K, void* stream);
 
 /* Gradients of ep_hip_grouped_gemm_bf16, dy in grouped order, rows 16-byte aligned.
  * _grad_rows (any N, the columns of dy from N to the next multiple of 8 readable and zero): row order[p] of dx (row p where order_dev is NULL) = dy[p] . w[g], zero for entries of no group.
- * _grad_weight (N a multiple of 8): dw[g] ([N][K], rows lddw and groups dw_group elements apart) = sum over the places of g of dy[p]^T x[order[p] / per_row];
+ * _grad_weight (N a multiple of 8): dw[g] ([N][K], rows lddw and groups dw_group elements apart) = sum over the places of g of dy[p]^T x[rows[p]];
  * zero for a group without rows. _column_sums: out[g][n] = sum of dy[p][n] (the bias's gradient). */
 int ep_hip_grouped_grad_rows_bf16(const void* dy_dev, int64_t lddy, const void* w_dev, int64_t ldw, int64_t w_group, void* dx_dev, int64_t lddx, int out_kind,
                                   const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N, int64_t K, void* stream);
 int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void* x_dev, int64_t ldx, int64_t x_rows, void* dw_dev, int64_t lddw, int64_t dw_group,
-                                    int out_kind, const int32_t* order_dev, int per_row, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
+                                    int out_kind, const int32_t* rows_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
                                     int64_t K, void* stream);
 int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int32_t* offsets_dev, int groups, int64_t N, void* out_dev, int out_kind, void* stream);
 

@@ -10,7 +10,7 @@ from entropack_amd.linear.groups import matrix
 def _plan(tokens=3, per_row=2, groups=4):
     entries = tokens * per_row
     index = torch.arange(entries, dtype=torch.int32)
-    return ep.RowGroups(index, torch.full((groups + 1,), entries, dtype=torch.int32), index.clone(), groups, tokens, per_row)
+    return ep.RowGroups(index, torch.full((groups + 1,), entries, dtype=torch.int32), index.clone(), index // per_row, groups, tokens, per_row)
 
 
 def _bf16(*shape):
@@ -168,29 +168,29 @@ def test_entry_points_refuse_bad_arguments():
     """Every check below fails before anything is launched, so no device is needed; the addresses are never followed."""
     lib, at, odd = hip.library(), 4096, 4104
     call = lambda name, good, **bad: getattr(lib, name)(*[bad.get(key, value) for key, value in good])
-    sort = [("ids", at), ("id_bytes", 8), ("entries", 5000), ("groups", 4), ("order", at), ("offsets", at), ("place", at), ("work", at), ("room", 1 << 20), ("stream", None)]
-    for bad in ({"ids": None}, {"id_bytes": 2}, {"entries": 0}, {"groups": 0}, {"order": None}, {"offsets": None}, {"place": None}, {"work": None}, {"room": 8}):
+    sort = [("ids", at), ("id_bytes", 8), ("entries", 5000), ("groups", 4), ("per_row", 1), ("order", at), ("offsets", at), ("place", at), ("rows", None), ("work", at), ("room", 1 << 20), ("stream", None)]
+    for bad in ({"ids": None}, {"id_bytes": 2}, {"entries": 0}, {"groups": 0}, {"per_row": 0}, {"order": None}, {"offsets": None}, {"place": None}, {"work": None}, {"room": 8}):
         assert call("ep_hip_group_rows", sort, **bad) == hip.EINVAL, bad
     for bad in ({"groups": 897}, {"entries": (1 << 30) + 1}):
         assert call("ep_hip_group_rows", sort, **bad) == hip.EUNSUPPORTED, bad
     assert lib.ep_hip_group_rows_workspace(10, 4) == 0 and lib.ep_hip_group_rows_workspace(1 << 20, 4) == 256 * 5 * 4
 
-    product = [("x", at), ("ldx", 16), ("x_rows", 4), ("w", at), ("ldw", 16), ("w_group", 64), ("bias", None), ("y", at), ("ldy", 4), ("kind", 0), ("order", at),
-               ("per_row", 2), ("offsets", at), ("entries", 8), ("groups", 2), ("N", 4), ("K", 16), ("stream", None)]
+    product = [("x", at), ("ldx", 16), ("x_rows", 4), ("w", at), ("ldw", 16), ("w_group", 64), ("bias", None), ("y", at), ("ldy", 4), ("kind", 0), ("rows", at),
+               ("offsets", at), ("entries", 8), ("groups", 2), ("N", 4), ("K", 16), ("stream", None)]
     for bad in ({"x": None}, {"x": odd}, {"w": odd}, {"w": None}, {"y": None}, {"ldx": 12}, {"ldx": 8}, {"ldw": 20}, {"w_group": 60}, {"w_group": -8}, {"ldy": 3}, {"kind": 3},
-                {"per_row": 0}, {"offsets": None}, {"entries": 0}, {"groups": 0}, {"N": 0}, {"K": 0}, {"K": 12}, {"order": None, "x_rows": 7}, {"N": 1 << 31}):
+                {"offsets": None}, {"entries": 0}, {"groups": 0}, {"N": 0}, {"K": 0}, {"K": 12}, {"rows": None, "x_rows": 7}, {"N": 1 << 31}):
         assert call("ep_hip_grouped_gemm_bf16", product, **bad) == hip.EINVAL, bad
     codes = [("x", at), ("ldx", 16), ("x_rows", 4), ("w", at), ("ldw", 16), ("w_group", 64), ("sx", at), ("sw", at), ("bias", None), ("y", at), ("ldy", 4), ("kind", 0),
-             ("order", at), ("per_row", 2), ("offsets", at), ("entries", 8), ("groups", 2), ("N", 4), ("K", 16), ("stream", None)]
+             ("rows", at), ("offsets", at), ("entries", 8), ("groups", 2), ("N", 4), ("K", 16), ("stream", None)]
     for bad in ({"sx": None}, {"sw": None}, {"ldx": 24}, {"K": 8}, {"w_group": 72}, {"kind": -1}):
         assert call("ep_hip_grouped_gemm_i8", codes, **bad) == hip.EINVAL, bad
     rows = [("dy", at), ("lddy", 8), ("w", at), ("ldw", 16), ("w_group", 128), ("dx", at), ("lddx", 16), ("kind", 0), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2),
             ("N", 8), ("K", 16), ("stream", None)]
     for bad in ({"dy": odd}, {"w": None}, {"dx": None}, {"lddx": 8}, {"N": 9}, {"K": 12}, {"lddy": 4}, {"offsets": None}):
         assert call("ep_hip_grouped_grad_rows_bf16", rows, **bad) == hip.EINVAL, bad
-    weight = [("dy", at), ("lddy", 8), ("x", at), ("ldx", 16), ("x_rows", 8), ("dw", at), ("lddw", 16), ("dw_group", 128), ("kind", 0), ("order", at), ("per_row", 1), ("offsets", at),
+    weight = [("dy", at), ("lddy", 8), ("x", at), ("ldx", 16), ("x_rows", 8), ("dw", at), ("lddw", 16), ("dw_group", 128), ("kind", 0), ("rows", at), ("offsets", at),
               ("entries", 8), ("groups", 2), ("N", 8), ("K", 16), ("stream", None)]
-    for bad in ({"dy": odd}, {"x": odd}, {"dw": None}, {"lddw": 8}, {"N": 4}, {"K": 12}, {"dw_group": -1}, {"order": None, "x_rows": 7}):
+    for bad in ({"dy": odd}, {"x": odd}, {"dw": None}, {"lddw": 8}, {"N": 4}, {"K": 12}, {"dw_group": -1}, {"rows": None, "x_rows": 7}):
         assert call("ep_hip_grouped_grad_weight_bf16", weight, **bad) == hip.EINVAL, bad
     sums = [("dy", at), ("lddy", 8), ("offsets", at), ("groups", 2), ("N", 8), ("out", at), ("kind", 0), ("stream", None)]
     for bad in ({"dy": None}, {"lddy": 4}, {"groups": 0}, {"N": 0}, {"out": None}, {"kind": 7}):

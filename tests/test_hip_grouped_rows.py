@@ -69,6 +69,7 @@ def test_group_rows(tokens, per_row, groups, kind):
         ids = _ids(tokens, per_row, groups, kind, dtype=dtype)
         plan = ep.group_rows(ids, groups)
         order, offsets, place = _plain_places(ids, groups)
+        assert torch.equal(plan.rows.cpu().long(), order // (per_row or 1))
         assert torch.equal(plan.order.cpu().long(), order) and torch.equal(plan.offsets.cpu().long(), offsets) and torch.equal(plan.place.cpu().long(), place)
         assert (plan.tokens, plan.per_row, plan.entries, plan.groups) == (tokens, per_row or 1, order.numel(), groups)
 
