@@ -45,22 +45,28 @@ static bool rows_in_pieces(const void* base, int64_t ld, int64_t K, int element_
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld >= K && (ld * element_bytes) % 16 == 0 && (K * element_bytes) % 16 == 0;
 }
 
+// `tile` rows and columns per block: the 128 x 128 kernel or the 256 x 256 one.
 template <bool INT8, int MODE, bool GATHER = true>
-static int launch_tile(const TileArgs& t, int64_t row_tiles, hipStream_t s) {
-  const int64_t blocks = row_tiles * ((t.columns + kTile - 1) / kTile);
+static int launch_tile(TileArgs t, int64_t row_tiles, int tile, hipStream_t s) {
+  t.tiles = tile_order(t.columns, tile);
+  const int64_t blocks = tile == kWideTile ? tile_blocks(t.tiles, row_tiles) : row_tiles * t.tiles.column_tiles;
   if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
-  const bool whole = MODE == kForward ? t.inner % 128 == 0 : (MODE == kGradRows && t.inner % 128 == 0 && t.columns % kTile == 0);
   const dim3 grid(static_cast<unsigned>(blocks));
-  if constexpr (MODE != kGradWeight) {
-    if (whole) {
-      hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, false, GATHER>), grid, dim3(256), 0, s, t);
-      EP_HIP_TRY(hipGetLastError());
-      return EP_HIP_OK;
-    }
+  const bool whole = MODE != kGradWeight && t.inner % (tile == kWideTile ? 256 : 128) == 0 && (MODE == kForward || t.columns % tile == 0);
+  if (tile == kWideTile) {
+    if (MODE != kGradWeight && whole) hipLaunchKernelGGL((grouped_wide_kernel<INT8, MODE, MODE == kGradWeight, GATHER>), grid, dim3(kWideThreads), 0, s, t);
+    else hipLaunchKernelGGL((grouped_wide_kernel<INT8, MODE, true, GATHER>), grid, dim3(kWideThreads), 0, s, t);
+  } else {
+    if (MODE != kGradWeight && whole) hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, MODE == kGradWeight, GATHER>), grid, dim3(256), 0, s, t);
+    else hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, true, GATHER>), grid, dim3(256), 0, s, t);
   }
-  hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, true, GATHER>), grid, dim3(256), 0, s, t);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
+}
+
+static int tile_for(int64_t entries, int groups, int64_t columns) {
+  (void)columns;
+  return entries / groups >= 256 ? kWideTile : kTile;
 }
 
 template <bool INT8>
@@ -71,7 +77,8 @@ static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
   t.lda_bytes = a.ldx_bytes, t.ldb_bytes = a.ldw_bytes, t.group_b_bytes = a.group_bytes, t.ldy = a.ldy;
   t.entries = a.entries, t.groups = a.groups, t.x_rows = a.x_rows, t.out_kind = a.out_kind;
   t.columns = a.N, t.inner = static_cast<int>(a.k_bytes);
-  return launch_tile<INT8, kForward>(t, most_row_tiles(a.entries, a.groups, kTile), s);
+  const int tile = tile_for(a.entries, a.groups, a.N);
+  return launch_tile<INT8, kForward>(t, most_row_tiles(a.entries, a.groups, tile), tile, s);
 }
 
 }  // namespace ep
@@ -119,7 +126,8 @@ int ep_hip_grouped_grad_rows_bf16(const void* dy_dev, int64_t lddy, const void* 
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldw * 2, t.group_b_bytes = w_group * 2, t.ldy = lddx;
   t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(entries), t.out_kind = out_kind;
   t.columns = static_cast<int>(K), t.inner = static_cast<int>(N * 2);
-  return launch_tile<false, kGradRows>(t, most_row_tiles(entries, groups, kTile), static_cast<hipStream_t>(stream));
+  const int tile = tile_for(entries, groups, K);
+  return launch_tile<false, kGradRows>(t, most_row_tiles(entries, groups, tile), tile, static_cast<hipStream_t>(stream));
 }
 
 int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void* x_dev, int64_t ldx, int64_t x_rows, void* dw_dev, int64_t lddw, int64_t dw_group,
@@ -134,9 +142,10 @@ int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldx * 2, t.ldy = lddw, t.group_y = dw_group;
   t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(x_rows), t.out_kind = out_kind;
   t.rows = static_cast<int>(N), t.columns = static_cast<int>(K);
-  const int64_t row_tiles = static_cast<int64_t>(groups) * ((N + kTile - 1) / kTile);
+  const int tile = tile_for(entries, groups, K);
+  const int64_t row_tiles = static_cast<int64_t>(groups) * ((N + tile - 1) / tile);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return rows_dev != nullptr ? launch_tile<false, kGradWeight, true>(t, row_tiles, s) : launch_tile<false, kGradWeight, false>(t, row_tiles, s);
+  return rows_dev != nullptr ? launch_tile<false, kGradWeight, true>(t, row_tiles, tile, s) : launch_tile<false, kGradWeight, false>(t, row_tiles, tile, s);
 }
 
 int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int32_t* offsets_dev, int groups, int64_t N, void* out_dev, int out_kind, void* stream) {
