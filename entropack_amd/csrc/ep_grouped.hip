@@ -48,17 +48,20 @@ static bool rows_in_pieces(const void* base, int64_t ld, int64_t K, int element_
 // `tile` rows and columns per block: the 128 x 128 kernel or the 256 x 256 one.
 template <bool INT8, int MODE, bool GATHER = true>
 static int launch_tile(TileArgs t, int64_t row_tiles, int tile, hipStream_t s) {
-  t.tiles = tile_order(t.columns, tile);
-  const int64_t blocks = tile == kWideTile ? tile_blocks(t.tiles, row_tiles) : row_tiles * t.tiles.column_tiles;
+  int device = 0;
+  EP_HIP_TRY(hipGetDevice(&device));
+  EP_HIP_TRY(hipDeviceGetAttribute(&t.compute_units, hipDeviceAttributeMultiprocessorCount, device));
+  const int64_t blocks = tile == kWideTile ? wide_blocks(row_tiles, t.columns, t.compute_units) : row_tiles * ((t.columns + kTile - 1) / kTile);
   if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
-  const bool whole = MODE != kGradWeight && t.inner % (tile == kWideTile ? 256 : 128) == 0 && (MODE == kForward || t.columns % tile == 0);
+  const bool whole = t.inner % 256 == 0 && (MODE == kForward || t.columns % tile == 0);
+  constexpr bool kAlways = MODE == kGradWeight;             // a group's rows are of any number
   if (tile == kWideTile) {
-    if (MODE != kGradWeight && whole) hipLaunchKernelGGL((grouped_wide_kernel<INT8, MODE, MODE == kGradWeight, GATHER>), grid, dim3(kWideThreads), 0, s, t);
-    else hipLaunchKernelGGL((grouped_wide_kernel<INT8, MODE, true, GATHER>), grid, dim3(kWideThreads), 0, s, t);
+    if (whole && !kAlways) hipLaunchKernelGGL((grouped_wide_kernel<INT8, MODE, kAlways, GATHER>), grid, dim3(kTileThreads), 0, s, t);
+    else hipLaunchKernelGGL((grouped_wide_kernel<INT8, MODE, true, GATHER>), grid, dim3(kTileThreads), 0, s, t);
   } else {
-    if (MODE != kGradWeight && whole) hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, MODE == kGradWeight, GATHER>), grid, dim3(256), 0, s, t);
-    else hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, true, GATHER>), grid, dim3(256), 0, s, t);
+    if (whole && !kAlways) hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, kAlways, GATHER>), grid, dim3(kTileThreads), 0, s, t);
+    else hipLaunchKernelGGL((grouped_tile_kernel<INT8, MODE, true, GATHER>), grid, dim3(kTileThreads), 0, s, t);
   }
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;

@@ -56,6 +56,17 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ off
   return {groups, static_cast<int>(first), static_cast<int>(left < tile_rows ? left : tile_rows), tile - before};
 }
 
+// How many tiles there are, those of no group included.
+__device__ __forceinline__ int64_t count_row_tiles(const int32_t* __restrict__ offsets, int groups, int entries, int tile_rows) {
+  const int lane = threadIdx.x & 63;
+  int mine = 0;
+  for (int g = lane; g < groups; g += 64) mine += (offsets[g + 1] - offsets[g] + tile_rows - 1) / tile_rows;
+  if (lane == 0) mine += (entries - offsets[groups] + tile_rows - 1) / tile_rows;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
+  return __builtin_amdgcn_readfirstlane(mine);
+}
+
 // The most tiles of `tile_rows` places that `entries` places in `groups` groups (and the places of none) make.
 inline int64_t most_row_tiles(int64_t entries, int groups, int tile_rows) {
   const int64_t parts = groups + 1 < entries ? groups + 1 : entries;          // every part may end with a tile of its own
