@@ -189,7 +189,8 @@ _SIGNATURES = {
         ctypes.c_void_p]),
     "ep_hip_low_rank_reduce": (ctypes.c_int, [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
-        ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
+        ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "ep_hip_low_rank_reduce_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64]),
     "ep_hip_low_rank_planes_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -44,7 +44,8 @@ struct TileArgs {
   int columns;                     // columns of y
   int inner;                       // forward, rows' gradient: the inner length in bytes of the row operand
   int compute_units;               // blocks of 256 x 256 tiles that run at a time
-};
+  int chunk;                       // weights' gradient, 128 x 128: 0, or places per chunk: y is then f32 [chunk][rows][columns], one matrix
+};                                 //   per chunk of a group's places (numbered like row tiles of `chunk` places)
 
 enum : int { kForward = 0, kGradRows = 1, kGradWeight = 2 };
 
@@ -131,7 +132,7 @@ __device__ __forceinline__ void store_wave_part(const TileArgs& g, Acc (&acc)[NI
 
 // What one block computes: rows [first_row, first_row + rows) of a group's rows (weights' gradient: of the weight) and columns n0 on.
 struct BlockTile {
-  int group;       // `groups`: rows of no group, which are written as zeros
+  int group;       // `groups`: rows of no group, which are written as zeros (weights' gradient: the matrix of y, a group's or a chunk's)
   int first;       // the place of the first row (weights' gradient: of the group)
   int rows;
   int m0;          // weights' gradient: first row
@@ -359,11 +360,19 @@ __device__ __forceinline__ bool find_block_tile(const TileArgs& g, int64_t at, i
   out.m0 = 0;
   if constexpr (MODE == kGradWeight) {
     const int row_tiles = (g.rows + tile - 1) / tile;
-    out.group = row_tile / row_tiles;
-    if (out.group >= g.groups) return false;
     out.m0 = row_tile % row_tiles * tile;
-    out.first = __builtin_amdgcn_readfirstlane(g.offsets[out.group]);
-    out.inner = __builtin_amdgcn_readfirstlane(g.offsets[out.group + 1]) - out.first;
+    if (g.chunk != 0) {
+      const RowTile found = find_row_tile(g.offsets, g.groups, g.entries, row_tile / row_tiles, g.chunk);
+      if (found.group < 0 || found.group == g.groups) return false;
+      out.group = row_tile / row_tiles;                     // where the result goes
+      out.first = found.first;
+      out.inner = found.rows;
+    } else {
+      out.group = row_tile / row_tiles;
+      if (out.group >= g.groups) return false;
+      out.first = __builtin_amdgcn_readfirstlane(g.offsets[out.group]);
+      out.inner = __builtin_amdgcn_readfirstlane(g.offsets[out.group + 1]) - out.first;
+    }
     out.rows = g.rows - out.m0 < tile ? g.rows - out.m0 : tile;
     out.steps = (out.inner + 63) / 64;
   } else {

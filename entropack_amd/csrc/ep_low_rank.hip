@@ -2,12 +2,12 @@
 //
 //   shrink   planes[p] = scale[a] x[order[p]] . down[a]^T      grouped_stream_kernel (ep_grouped.hpp), bound by reading x
 //   expand   out[order[p]] = y[order[p]] + planes[p] . up[a]^T   low_rank_expand_kernel, bound by reading y and writing out
-//   reduce   sum_p planes[p]^T q[order[p]]                     low_rank_reduce_kernel: the gradients of down (q = x, planes of the
+//   reduce   sum_p planes[p]^T q[order[p]]                     grouped_tile_kernel, low_rank_finish_kernel: the gradients of down (q = x, planes of the
 //                                                              output's gradient) and of up (q = the output's gradient)
 // The narrow rows in between ("planes") are kept as two bf16 parts, value and remainder, so that the second product loses
 // nothing that the output's own rounding would show: each rounding is off by at most 2^-8 of what it
 // rounds, so the two parts together by at most 2^-16 of the f32 value.
-#include "ep_grouped.hpp"
+#include "ep_grouped_tile.hpp"
 
 namespace ep {
 
@@ -116,33 +116,61 @@ __global__ __launch_bounds__(256) void low_rank_expand_kernel(LowRankArgs a) {
   }
 }
 
-// sum over a group's places of planes[p][e] q[order[p]][n] for all e < rank (value + remainder): out[g][e][n], or
-// out[g][n][e] when transposed. In its simplest form: a block takes 256 columns and 8 ranks of one group.
-__global__ __launch_bounds__(256) void low_rank_reduce_kernel(const uint16_t* __restrict__ planes, int padded, int rank, const uint16_t* __restrict__ q, int64_t ldq,
-                                                              const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int rows, int width,
-                                                              uint16_t* __restrict__ out, int transposed) {
-  const int column_tiles = (width + 255) / 256, rank_tiles = (rank + 7) / 8;
-  const int column = static_cast<int>(blockIdx.x % column_tiles) * 256 + threadIdx.x;
-  const int at = static_cast<int>(blockIdx.x / column_tiles);
-  const int e0 = at % rank_tiles * 8, group = at / rank_tiles;
-  const int first = offsets[group], last = offsets[group + 1];
-  if (column >= width) return;
-  float sum[8] = {};
-  for (int p = first; p < last; ++p) {
-    int row = order[p];
-    row = row < rows ? row : rows - 1;
-    const float v = __uint_as_float(static_cast<uint32_t>(q[row * ldq + column]) << 16);
-    const uint16_t* plane = planes + static_cast<int64_t>(p) * (2 * padded) + e0;
+// sum over a group's places of planes[p][e] q[order[p]][n] for all e < rank (value + remainder): out[g][e][n], or out[g][n][e] when
+// transposed. The products are the weights' gradient of ep_grouped_tile.hpp with the planes as left operand. They are bound by
+// reading q, and the groups alone make too few tiles to fill the card, so the places of every group are divided into chunks, each
+// chunk writes its f32 sums to a matrix of its own, and this kernel adds a group's chunks in their order and rounds once.
+// A block takes 64 columns of one group, 64 ranks at a time.
+__global__ __launch_bounds__(256) void low_rank_finish_kernel(const float* __restrict__ parts, int chunk, int padded, int rank, const int32_t* __restrict__ offsets,
+                                                              int width, uint16_t* __restrict__ out, int transposed) {
+  __shared__ uint16_t turned[64][66];
+  const int column_tiles = (width + 63) / 64;
+  const int group = static_cast<int>(blockIdx.x / column_tiles), n0 = static_cast<int>(blockIdx.x % column_tiles) * 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // The chunks of the groups before this one, and this one's.
+  int before = 0;
+  for (int g = lane; g < group; g += 64) before += (offsets[g + 1] - offsets[g] + chunk - 1) / chunk;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float h = __uint_as_float(static_cast<uint32_t>(plane[i]) << 16) + __uint_as_float(static_cast<uint32_t>(plane[padded + i]) << 16);
-      sum[i] = __builtin_fmaf(h, v, sum[i]);
+  for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d);
+  const int chunks = (offsets[group + 1] - offsets[group] + chunk - 1) / chunk;
+  const int64_t matrix = static_cast<int64_t>(2 * padded) * width;
+  const float* from = parts + before * matrix;
+  const int n = n0 + lane;
+  for (int e0 = 0; e0 < rank; e0 += 64) {
+    const int ranks = rank - e0 < 64 ? rank - e0 : 64;
+    for (int e = wave; e < ranks; e += 4) {
+      float sum = 0.0f;
+      if (n < width) {
+        const float* high = from + static_cast<int64_t>(e0 + e) * width + n;
+        const float* low = high + static_cast<int64_t>(padded) * width;
+#pragma unroll 4
+        for (int c = 0; c < chunks; ++c) sum += high[c * matrix] + low[c * matrix];
+      }
+      const uint16_t bits = static_cast<uint16_t>(bf16_bits_of(sum));
+      if (transposed) turned[lane][e] = bits;
+      else if (n < width) out[(static_cast<int64_t>(group) * rank + e0 + e) * width + n] = bits;
+    }
+    if (transposed) {
+      __syncthreads();
+      const int columns = width - n0 < 64 ? width - n0 : 64;
+      for (int cell = threadIdx.x; cell < columns * ranks; cell += 256)
+        out[(static_cast<int64_t>(group) * width + n0 + cell / ranks) * rank + e0 + cell % ranks] = turned[cell / ranks][cell % ranks];
+      __syncthreads();
     }
   }
-  for (int i = 0; i < 8 && e0 + i < rank; ++i) {
-    const int64_t to = transposed ? (static_cast<int64_t>(group) * width + column) * rank + e0 + i : (static_cast<int64_t>(group) * rank + e0 + i) * width + column;
-    out[to] = static_cast<uint16_t>(bf16_bits_of(sum[i]));
-  }
+}
+
+// Places per chunk: about 1024 tiles in all, at least 128 places each (a chunk of fewer does not outlast its own prologue).
+static int reduce_chunk(int64_t entries, int64_t rank, int64_t width) {
+  const int64_t tiles = ((width + kTile - 1) / kTile) * (((rank + 15) / 16 * 32 + kTile - 1) / kTile);
+  const int64_t chunks = tiles >= 1024 ? 1 : 1024 / tiles;
+  int64_t chunk = (entries + chunks - 1) / chunks;
+  chunk = chunk < 128 ? 128 : (chunk + 63) / 64 * 64;
+  return static_cast<int>(chunk < (1 << 30) ? chunk : 1 << 30);
+}
+
+static int64_t reduce_chunks(int64_t entries, int groups, int chunk) {       // the most there can be
+  return entries / chunk + (groups < entries ? groups : entries);
 }
 
 static bool low_rank_valid(const int32_t* order, const int32_t* offsets, int64_t entries, int groups, int64_t rows, int64_t rank, int64_t width) {
@@ -198,16 +226,34 @@ int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t l
   return EP_HIP_OK;
 }
 
-int ep_hip_low_rank_reduce(const void* planes_dev, const void* q_dev, int64_t ldq, void* out_dev, int transposed, const int32_t* order_dev, const int32_t* offsets_dev,
-                           int64_t entries, int groups, int64_t rank, int64_t width, void* stream) {
+size_t ep_hip_low_rank_reduce_workspace(int64_t entries, int groups, int64_t rank, int64_t width) {
   using namespace ep;
-  if (planes_dev == nullptr || q_dev == nullptr || out_dev == nullptr || !low_rank_valid(order_dev, offsets_dev, entries, groups, entries, rank, width)) return EP_HIP_EINVAL;
-  if (ldq < width) return EP_HIP_EINVAL;
-  const int64_t blocks = static_cast<int64_t>(groups) * ((rank + 7) / 8) * ((width + 255) / 256);
-  if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
-  hipLaunchKernelGGL(low_rank_reduce_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const uint16_t*>(planes_dev),
-                     static_cast<int>((rank + 15) / 16 * 16), static_cast<int>(rank), static_cast<const uint16_t*>(q_dev), ldq, order_dev, offsets_dev, static_cast<int>(entries),
-                     static_cast<int>(width), static_cast<uint16_t*>(out_dev), transposed);
+  if (entries <= 0 || groups <= 0 || rank <= 0 || width <= 0) return 0;
+  return static_cast<size_t>(reduce_chunks(entries, groups, reduce_chunk(entries, rank, width))) * static_cast<size_t>((rank + 15) / 16 * 32) * static_cast<size_t>(width) * 4;
+}
+
+int ep_hip_low_rank_reduce(const void* planes_dev, const void* q_dev, int64_t ldq, void* out_dev, int transposed, const int32_t* order_dev, const int32_t* offsets_dev,
+                           int64_t entries, int groups, int64_t rank, int64_t width, void* workspace_dev, size_t workspace_bytes, void* stream) {
+  using namespace ep;
+  if (planes_dev == nullptr || q_dev == nullptr || out_dev == nullptr || workspace_dev == nullptr) return EP_HIP_EINVAL;
+  if (!low_rank_valid(order_dev, offsets_dev, entries, groups, entries, rank, width)) return EP_HIP_EINVAL;
+  const int64_t readable = (width + 7) / 8 * 8;
+  if (ldq < readable || ldq % 8 != 0 || reinterpret_cast<uintptr_t>(q_dev) % 16 != 0 || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
+  if (reinterpret_cast<uintptr_t>(workspace_dev) % 16 != 0 || workspace_bytes < ep_hip_low_rank_reduce_workspace(entries, groups, rank, width)) return EP_HIP_EINVAL;
+  const int padded = static_cast<int>((rank + 15) / 16 * 16);
+  TileArgs t = {};
+  t.a = static_cast<const uint8_t*>(planes_dev), t.b = static_cast<const uint8_t*>(q_dev), t.y = workspace_dev, t.row_of = order_dev, t.offsets = offsets_dev;
+  t.lda_bytes = padded * int64_t{4}, t.ldb_bytes = ldq * 2, t.ldy = width, t.group_y = 2 * padded * width;
+  t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(entries), t.out_kind = kOutF32;
+  t.rows = 2 * padded, t.columns = static_cast<int>(width), t.chunk = reduce_chunk(entries, rank, width);
+  const int64_t blocks = reduce_chunks(entries, groups, t.chunk) * ((t.rows + kTile - 1) / kTile) * ((width + kTile - 1) / kTile);
+  const int64_t finish = groups * ((width + 63) / 64);
+  if (blocks > 0x7FFFFFFF || finish > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL((grouped_tile_kernel<false, kGradWeight, true, true>), dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0, s, t);
+  EP_HIP_TRY(hipGetLastError());
+  hipLaunchKernelGGL(low_rank_finish_kernel, dim3(static_cast<unsigned>(finish)), dim3(256), 0, s, static_cast<const float*>(workspace_dev), t.chunk, padded,
+                     static_cast<int>(rank), offsets_dev, static_cast<int>(width), static_cast<uint16_t*>(out_dev), transposed);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
 }

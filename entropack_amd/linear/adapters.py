@@ -47,9 +47,11 @@ def _reduce(planes, rank: int, rows, transposed: bool, groups: RowGroups) -> tor
     rows = matrix(rows, 8)
     out = torch.empty((groups.groups, width, rank) if transposed else (groups.groups, rank, width), dtype=torch.bfloat16, device=planes.device)
     with torch.cuda.device(planes.device):
-        _hip.check("ep_hip_low_rank_reduce", _hip.library().ep_hip_low_rank_reduce(
+        lib = _hip.library()
+        workspace = torch.empty(lib.ep_hip_low_rank_reduce_workspace(groups.entries, groups.groups, rank, width), dtype=torch.uint8, device=planes.device)
+        _hip.check("ep_hip_low_rank_reduce", lib.ep_hip_low_rank_reduce(
             planes.data_ptr(), rows.data_ptr(), rows.stride(0), out.data_ptr(), int(transposed), groups.order.data_ptr(), groups.offsets.data_ptr(),
-            groups.entries, groups.groups, rank, width, _hip.current_stream(planes.device)))
+            groups.entries, groups.groups, rank, width, workspace.data_ptr(), workspace.numel(), _hip.current_stream(planes.device)))
     return out
 
 

@@ -467,13 +467,15 @@ int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int3
  * [0, padded) the rounded value, [padded, 2 padded) the rounded remainder, padded = rank rounded up to 16;
  * ep_hip_low_rank_planes_bytes bytes, 16-byte aligned. down: [groups][rank][K], K a multiple of 8, 16-byte aligned rows.
  * _expand: out[order[p]] = y[order[p]] + planes[p] . up[g]^T (bf16; y NULL: zero; rows of no group: y). up: [groups][N][rank].
- * _reduce: out[g][e][n] (or, transposed, out[g][n][e]; bf16, contiguous) = sum over the places of g of planes[p][e] q[order[p]][n]. */
+ * _reduce: out[g][e][n] (or, transposed, out[g][n][e]; bf16, contiguous) = sum over the places of g of planes[p][e] q[order[p]][n]; q
+ * 16-byte aligned, ldq a multiple of 8, the columns from width to the next multiple of 8 readable; workspace 16-byte aligned. */
 int ep_hip_low_rank_shrink(const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group, const float* scale_dev, void* planes_dev,
                            const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t K, void* stream);
 int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t ldu, int64_t up_group, const void* y_dev, int64_t ldy, void* out_dev, int64_t ldo,
                            const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t N, void* stream);
 int ep_hip_low_rank_reduce(const void* planes_dev, const void* q_dev, int64_t ldq, void* out_dev, int transposed, const int32_t* order_dev, const int32_t* offsets_dev,
-                           int64_t entries, int groups, int64_t rank, int64_t width, void* stream);
+                           int64_t entries, int groups, int64_t rank, int64_t width, void* workspace_dev, size_t workspace_bytes, void* stream);
+size_t ep_hip_low_rank_reduce_workspace(int64_t entries, int groups, int64_t rank, int64_t width);
 size_t ep_hip_low_rank_planes_bytes(int64_t entries, int64_t rank);
 
 #ifdef __cplusplus

@@ -204,8 +204,9 @@ def test_entry_points_refuse_bad_arguments():
               ("N", 16), ("stream", None)]
     for bad in ({"planes": None}, {"up": None}, {"out": None}, {"ldu": 3}, {"ldy": 8}, {"ldo": 8}, {"group": -1}, {"N": 0}, {"offsets": None}):
         assert call("ep_hip_low_rank_expand", expand, **bad) == hip.EINVAL, bad
-    reduce = [("planes", at), ("q", at), ("ldq", 16), ("out", at), ("transposed", 0), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4), ("width", 16), ("stream", None)]
-    for bad in ({"planes": None}, {"q": None}, {"out": None}, {"ldq": 8}, {"rank": 0}, {"width": 0}):
+    reduce = [("planes", at), ("q", at), ("ldq", 16), ("out", at), ("transposed", 0), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4), ("width", 16), ("work", at),
+              ("room", 1 << 30), ("stream", None)]
+    for bad in ({"planes": None}, {"q": None}, {"out": None}, {"ldq": 8}, {"ldq": 20}, {"rank": 0}, {"width": 0}, {"q": odd}, {"work": None}, {"room": 16}):
         assert call("ep_hip_low_rank_reduce", reduce, **bad) == hip.EINVAL, bad
 
     combine = [("y", at), ("kind", 0), ("ldy", 8), ("place", at), ("kept", at), ("weight", at), ("weight_kind", 2), ("per_row", 2), ("tokens", 4), ("width", 8), ("out", at), ("ldo", 8), ("stream", None)]
