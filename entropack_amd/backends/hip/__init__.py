@@ -267,3 +267,17 @@ def pointer(tensor: torch.Tensor) -> int | None:
 
 def current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(name: str, device: torch.device, *arguments) -> None:
+    """Calls an entry point whose last argument is the stream on `device` and torch's current stream there. For calls whose time
+    is that of the host: the device guard is taken only where another device is current (1.3 us), the stream's handle is
+    asked for without a Stream object around it (1.9 us)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = getattr(library(), name)(*arguments, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(library(), name)(*arguments, torch._C._cuda_getCurrentRawStream(index))
+    if status != OK:
+        check(name, status)

@@ -124,7 +124,14 @@ __device__ __forceinline__ void store_wave_part(const TileArgs& g, Acc (&acc)[NI
           packed = make_uint4(half_bits(lo.x) | half_bits(lo.y) << 16, half_bits(lo.z) | half_bits(lo.w) << 16, half_bits(hi.x) | half_bits(hi.y) << 16,
                               half_bits(hi.z) | half_bits(hi.w) << 16);
         }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.y) + row_offset(row0 + row) + n) = packed;
+        uint16_t* to = static_cast<uint16_t*>(g.y) + row_offset(row0 + row) + n;
+        if constexpr (MODE == kGradWeight) {
+          // Gradients of whole weights are read again much later, if at all from a cache: 580 -> 547 us for eight of 4096 x 4096.
+          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+          __builtin_nontemporal_store(u32x4{packed.x, packed.y, packed.z, packed.w}, reinterpret_cast<u32x4*>(to));
+        } else {
+          *reinterpret_cast<uint4*>(to) = packed;
+        }
       }
     }
   }

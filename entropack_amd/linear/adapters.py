@@ -19,25 +19,23 @@ def _shrink(x, down, scale, groups: RowGroups) -> torch.Tensor:
     rank = down.shape[1]
     planes = torch.empty(groups.entries, 2 * (-(-rank // 16) * 16), dtype=torch.bfloat16, device=x.device)
     rows, narrow = matrix(x, 8), matrix(down, 8)
-    with torch.cuda.device(x.device):
-        _hip.check("ep_hip_low_rank_shrink", _hip.library().ep_hip_low_rank_shrink(
-            rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0), None if scale is None else scale.data_ptr(),
-            planes.data_ptr(), groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, rows.shape[1],
-            _hip.current_stream(x.device)))
+    _hip.launch("ep_hip_low_rank_shrink", x.device,
+                rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0), None if scale is None else scale.data_ptr(),
+                planes.data_ptr(), groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, rows.shape[1])
     return planes
 
 
 def _expand(planes, up, y, groups: RowGroups) -> torch.Tensor:
     """y + planes up[a]^T, rows of no group as they are in y (zero where y is None)."""
     outer, rank = up.shape[1], up.shape[2]
+    if not (up.stride(2) == 1 and up.stride(1) >= rank and up.stride(0) >= outer * up.stride(1)):
+        up = up.contiguous()
     out = torch.empty(groups.entries, outer, dtype=torch.bfloat16, device=planes.device)
     if y is not None and not (y.stride(1) == 1 and y.stride(0) >= outer):
         y = y.contiguous()
-    with torch.cuda.device(planes.device):
-        _hip.check("ep_hip_low_rank_expand", _hip.library().ep_hip_low_rank_expand(
-            planes.data_ptr(), up.data_ptr(), up.stride(1), up.stride(0), None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
-            out.data_ptr(), outer, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, outer,
-            _hip.current_stream(planes.device)))
+    _hip.launch("ep_hip_low_rank_expand", planes.device,
+                planes.data_ptr(), up.data_ptr(), up.stride(1), up.stride(0), None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
+                out.data_ptr(), outer, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, outer)
     return out
 
 
@@ -46,20 +44,19 @@ def _reduce(planes, rank: int, rows, transposed: bool, groups: RowGroups) -> tor
     width = rows.shape[1]
     rows = matrix(rows, 8)
     out = torch.empty((groups.groups, width, rank) if transposed else (groups.groups, rank, width), dtype=torch.bfloat16, device=planes.device)
-    with torch.cuda.device(planes.device):
-        lib = _hip.library()
-        workspace = torch.empty(lib.ep_hip_low_rank_reduce_workspace(groups.entries, groups.groups, rank, width), dtype=torch.uint8, device=planes.device)
-        _hip.check("ep_hip_low_rank_reduce", lib.ep_hip_low_rank_reduce(
-            planes.data_ptr(), rows.data_ptr(), rows.stride(0), out.data_ptr(), int(transposed), groups.order.data_ptr(), groups.offsets.data_ptr(),
-            groups.entries, groups.groups, rank, width, workspace.data_ptr(), workspace.numel(), _hip.current_stream(planes.device)))
+    room = _hip.library().ep_hip_low_rank_reduce_workspace(groups.entries, groups.groups, rank, width)
+    workspace = torch.empty(room, dtype=torch.uint8, device=planes.device)
+    _hip.launch("ep_hip_low_rank_reduce", planes.device,
+                planes.data_ptr(), rows.data_ptr(), rows.stride(0), out.data_ptr(), int(transposed), groups.order.data_ptr(), groups.offsets.data_ptr(),
+                groups.entries, groups.groups, rank, width, workspace.data_ptr(), room)
     return out
 
 
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, down, up, scale, groups):
-        planes = _shrink(x.detach(), down.detach(), scale, groups)
-        out = _expand(planes, up.detach().contiguous(), y.detach(), groups)
+        planes = _shrink(x, down, scale, groups)
+        out = _expand(planes, up, y, groups)
         ctx.groups = groups
         ctx.save_for_backward(x, down, up, scale, planes if ctx.needs_input_grad[3] else None)
         return out
@@ -118,11 +115,13 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
             raise ValueError(f"low_rank_update takes one scale per adapter, got shape {tuple(scale.shape)}")
         if scale.requires_grad:
             raise ValueError("low_rank_update gives no gradient of the scale: detach it")
-        scale = scale.float().contiguous()
+        scale = scale if scale.dtype == torch.float32 and scale.is_contiguous() else scale.float().contiguous()
     device_of("low_rank_update", y, x, down, up, groups.order, scale)
     if groups.tokens == 0:
         return y + (x.sum() + down.sum() + up.sum()) * 0
-    return _LowRankUpdate.apply(y, x, down, up, scale, groups)
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or down.requires_grad or up.requires_grad):
+        return _LowRankUpdate.apply(y, x, down, up, scale, groups)
+    return _expand(_shrink(x, down, scale, groups), up, y, groups)
 
 
 class AdaptedLinear(torch.nn.Module):

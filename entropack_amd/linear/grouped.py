@@ -41,12 +41,11 @@ def _forward(x, weight, bias, groups: RowGroups, x_grouped: bool) -> torch.Tenso
     if y.numel():
         rows, w = matrix(x, 8), matrix(weight, 8)
         ready = None if bias is None else bias.contiguous()
-        with torch.cuda.device(x.device):
-            _hip.check("ep_hip_grouped_gemm_bf16", _hip.library().ep_hip_grouped_gemm_bf16(
-                rows.data_ptr(), rows.stride(0), rows.shape[0], w.data_ptr(), w.stride(1), w.stride(0),
-                None if ready is None else ready.data_ptr(), y.data_ptr(), outer, _hip.FLOAT_KINDS[torch.bfloat16],
-                None if x_grouped else groups.rows.data_ptr(), groups.offsets.data_ptr(), groups.entries,
-                groups.groups, outer, rows.shape[1], _hip.current_stream(x.device)))
+        _hip.launch("ep_hip_grouped_gemm_bf16", x.device,
+                    rows.data_ptr(), rows.stride(0), rows.shape[0], w.data_ptr(), w.stride(1), w.stride(0),
+                    None if ready is None else ready.data_ptr(), y.data_ptr(), outer, _hip.FLOAT_KINDS[torch.bfloat16],
+                    None if x_grouped else groups.rows.data_ptr(), groups.offsets.data_ptr(), groups.entries,
+                    groups.groups, outer, rows.shape[1])
     return y
 
 
@@ -60,11 +59,10 @@ def _grad_rows(grad, weight, groups: RowGroups, x_grouped: bool) -> torch.Tensor
         dy, w = matrix(grad, 8), matrix(weight, 8)
         if w.shape[2] != inner:                                  # padded columns would be written past the rows of out
             out = torch.empty(groups.entries, w.shape[2], dtype=out.dtype, device=grad.device)
-        with torch.cuda.device(grad.device):
-            _hip.check("ep_hip_grouped_grad_rows_bf16", _hip.library().ep_hip_grouped_grad_rows_bf16(
-                dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(1), w.stride(0), out.data_ptr(), out.stride(0),
-                _hip.FLOAT_KINDS[out.dtype], None if x_grouped else groups.order.data_ptr(), groups.offsets.data_ptr(),
-                groups.entries, groups.groups, w.shape[1], w.shape[2], _hip.current_stream(grad.device)))
+        _hip.launch("ep_hip_grouped_grad_rows_bf16", grad.device,
+                    dy.data_ptr(), dy.stride(0), w.data_ptr(), w.stride(1), w.stride(0), out.data_ptr(), out.stride(0),
+                    _hip.FLOAT_KINDS[out.dtype], None if x_grouped else groups.order.data_ptr(), groups.offsets.data_ptr(),
+                    groups.entries, groups.groups, w.shape[1], w.shape[2])
     if summed:
         out = sum_entries(out, groups.tokens, groups.per_row)
     return out if out.shape[1] == inner else out[:, :inner].contiguous()
@@ -76,11 +74,10 @@ def _grad_weight(grad, x, weight, groups: RowGroups, x_grouped: bool) -> torch.T
     dy, rows = matrix(grad, 8), matrix(x, 8)
     outer, inner = dy.shape[1], rows.shape[1]
     out = torch.empty(groups.groups, outer, inner, dtype=torch.bfloat16, device=grad.device)
-    with torch.cuda.device(grad.device):
-        _hip.check("ep_hip_grouped_grad_weight_bf16", _hip.library().ep_hip_grouped_grad_weight_bf16(
-            dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), rows.shape[0], out.data_ptr(), inner, outer * inner,
-            _hip.FLOAT_KINDS[torch.bfloat16], None if x_grouped else groups.rows.data_ptr(),
-            groups.offsets.data_ptr(), groups.entries, groups.groups, outer, inner, _hip.current_stream(grad.device)))
+    _hip.launch("ep_hip_grouped_grad_weight_bf16", grad.device,
+                dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), rows.shape[0], out.data_ptr(), inner, outer * inner,
+                _hip.FLOAT_KINDS[torch.bfloat16], None if x_grouped else groups.rows.data_ptr(),
+                groups.offsets.data_ptr(), groups.entries, groups.groups, outer, inner)
     return out if tuple(out.shape) == tuple(weight.shape) else out[:, :weight.shape[1], :weight.shape[2]].contiguous()
 
 
@@ -90,10 +87,9 @@ def _grad_bias(grad, groups: RowGroups) -> torch.Tensor:
         return torch.zeros(groups.groups, outer, dtype=torch.bfloat16, device=grad.device)
     dy = grad if grad.stride(1) == 1 and grad.stride(0) >= outer else grad.contiguous()
     out = torch.empty(groups.groups, outer, dtype=torch.bfloat16, device=grad.device)
-    with torch.cuda.device(grad.device):
-        _hip.check("ep_hip_grouped_column_sums_bf16", _hip.library().ep_hip_grouped_column_sums_bf16(
-            dy.data_ptr(), dy.stride(0), groups.offsets.data_ptr(), groups.groups, outer, out.data_ptr(),
-            _hip.FLOAT_KINDS[torch.bfloat16], _hip.current_stream(grad.device)))
+    _hip.launch("ep_hip_grouped_column_sums_bf16", grad.device,
+                dy.data_ptr(), dy.stride(0), groups.offsets.data_ptr(), groups.groups, outer, out.data_ptr(),
+                _hip.FLOAT_KINDS[torch.bfloat16])
     return out
 
 
@@ -102,7 +98,7 @@ class _GroupedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, groups, x_grouped):
         ctx.groups, ctx.x_grouped = groups, x_grouped
         ctx.save_for_backward(x, weight)
-        return _forward(x.detach(), weight.detach(), None if bias is None else bias.detach(), groups, x_grouped)
+        return _forward(x, weight, bias, groups, x_grouped)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -134,7 +130,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
         if tensor is not None and tensor.dtype != torch.bfloat16:
             raise TypeError(f"grouped_linear takes bfloat16 operands, got {name} in {tensor.dtype}")
     device_of("grouped_linear", x, weight, groups.order, bias)
-    return _GroupedLinear.apply(x, weight, bias, groups, x_grouped)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _GroupedLinear.apply(x, weight, bias, groups, x_grouped)
+    return _forward(x, weight, bias, groups, x_grouped)
 
 
 def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, x_scale: torch.Tensor, weight_scale: torch.Tensor,
@@ -163,12 +161,11 @@ def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups
     rows, w = matrix(x, 16), matrix(weight, 16)
     ready = None if bias is None else bias.detach().to(out_dtype).contiguous()
     scale_x, scale_w = x_scale.detach().float().contiguous(), weight_scale.detach().float().contiguous()
-    with torch.cuda.device(device):
-        _hip.check("ep_hip_grouped_gemm_i8", _hip.library().ep_hip_grouped_gemm_i8(
-            rows.data_ptr(), rows.stride(0), rows.shape[0], w.data_ptr(), w.stride(1), w.stride(0), scale_x.data_ptr(), scale_w.data_ptr(),
-            None if ready is None else ready.data_ptr(), y.data_ptr(), outer, _hip.FLOAT_KINDS[out_dtype],
-            None if x_grouped else groups.rows.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups,
-            outer, rows.shape[1], _hip.current_stream(device)))
+    _hip.launch("ep_hip_grouped_gemm_i8", device,
+                rows.data_ptr(), rows.stride(0), rows.shape[0], w.data_ptr(), w.stride(1), w.stride(0), scale_x.data_ptr(), scale_w.data_ptr(),
+                None if ready is None else ready.data_ptr(), y.data_ptr(), outer, _hip.FLOAT_KINDS[out_dtype],
+                None if x_grouped else groups.rows.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups,
+                outer, rows.shape[1])
     return y
 
 

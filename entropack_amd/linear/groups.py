@@ -107,13 +107,11 @@ def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
         return RowGroups(order, torch.zeros(groups + 1, dtype=torch.int32, device=device), place, rows, groups, tokens, per_row)
     offsets = torch.empty(groups + 1, dtype=torch.int32, device=device)
     flat = ids.contiguous()
-    with torch.cuda.device(device):
-        lib = _hip.library()
-        room = lib.ep_hip_group_rows_workspace(entries, groups)
-        workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-        _hip.check("ep_hip_group_rows", lib.ep_hip_group_rows(
-            flat.data_ptr(), flat.element_size(), entries, groups, per_row, order.data_ptr(), offsets.data_ptr(), place.data_ptr(),
-            rows.data_ptr() if per_row > 1 else None, None if workspace is None else workspace.data_ptr(), room, _hip.current_stream(device)))
+    room = _hip.library().ep_hip_group_rows_workspace(entries, groups)
+    workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    _hip.launch("ep_hip_group_rows", device,
+                flat.data_ptr(), flat.element_size(), entries, groups, per_row, order.data_ptr(), offsets.data_ptr(), place.data_ptr(),
+                rows.data_ptr() if per_row > 1 else None, None if workspace is None else workspace.data_ptr(), room)
     return RowGroups(order, offsets, place, rows, groups, tokens, per_row)
 
 
@@ -126,10 +124,9 @@ def sum_entries(rows: torch.Tensor, tokens: int, per_row: int) -> torch.Tensor:
     """[entries, width] rows in the order of the entries (f32 or bf16) added up per token, rounded to bf16 once."""
     out = torch.empty(tokens, rows.shape[1], dtype=torch.bfloat16, device=rows.device)
     if out.numel():
-        with torch.cuda.device(rows.device):
-            _hip.check("ep_hip_combine_rows", _hip.library().ep_hip_combine_rows(
-                rows.data_ptr(), _ROW_KINDS[rows.dtype], rows.stride(0), None, None, None, 0, per_row, tokens, rows.shape[1],
-                out.data_ptr(), out.stride(0), _hip.current_stream(rows.device)))
+        _hip.launch("ep_hip_combine_rows", rows.device,
+                    rows.data_ptr(), _ROW_KINDS[rows.dtype], rows.stride(0), None, None, None, 0, per_row, tokens, rows.shape[1],
+                    out.data_ptr(), out.stride(0))
     return out
 
 
@@ -138,21 +135,24 @@ def _rows_of(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.stride(1) == 1 and tensor.stride(0) >= tensor.shape[1] else tensor.contiguous()
 
 
+def _combine(y, weight, groups: RowGroups) -> torch.Tensor:
+    rows = _rows_of(y)
+    ready = None if weight is None else weight.contiguous()
+    out = torch.empty(groups.tokens, y.shape[1], dtype=torch.bfloat16, device=y.device)
+    if out.numel():
+        _hip.launch("ep_hip_combine_rows", y.device,
+                    rows.data_ptr(), _ROW_KINDS[torch.bfloat16], rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
+                    None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
+                    groups.tokens, rows.shape[1], out.data_ptr(), out.stride(0))
+    return out
+
+
 class _CombineRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weight, groups):
-        rows = _rows_of(y.detach())
-        ready = None if weight is None else weight.detach().contiguous()
-        out = torch.empty(groups.tokens, y.shape[1], dtype=torch.bfloat16, device=y.device)
-        if out.numel():
-            with torch.cuda.device(y.device):
-                _hip.check("ep_hip_combine_rows", _hip.library().ep_hip_combine_rows(
-                    rows.data_ptr(), _ROW_KINDS[torch.bfloat16], rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
-                    None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
-                    groups.tokens, rows.shape[1], out.data_ptr(), out.stride(0), _hip.current_stream(y.device)))
         ctx.groups = groups
         ctx.save_for_backward(y, weight)
-        return out
+        return _combine(y, weight, groups)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -163,12 +163,11 @@ class _CombineRows(torch.autograd.Function):
         grad_weight = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_weight else None
         if y.numel():
             rows, ready, slope = _rows_of(y), None if weight is None else weight.contiguous(), _rows_of(grad)
-            with torch.cuda.device(y.device):
-                _hip.check("ep_hip_combine_rows_grad", _hip.library().ep_hip_combine_rows_grad(
-                    slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
-                    None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
-                    groups.tokens, rows.shape[1], None if grad_y is None else grad_y.data_ptr(), rows.shape[1],
-                    None if grad_weight is None else grad_weight.data_ptr(), _hip.current_stream(y.device)))
+            _hip.launch("ep_hip_combine_rows_grad", y.device,
+                        slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
+                        None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
+                        groups.tokens, rows.shape[1], None if grad_y is None else grad_y.data_ptr(), rows.shape[1],
+                        None if grad_weight is None else grad_weight.data_ptr())
         elif grad_weight is not None:
             grad_weight.zero_()
         return grad_y, grad_weight, None
@@ -197,7 +196,9 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weight: torch.Tensor | None
         if tuple(weight.shape) not in ({(groups.tokens, groups.per_row)} | ({(groups.tokens,)} if groups.per_row == 1 else set())):
             raise ValueError(f"combine_rows takes weights of shape {(groups.tokens, groups.per_row)}, got {tuple(weight.shape)}")
     device_of("combine_rows", y, groups.order, weight)
-    return _CombineRows.apply(y, weight, groups)
+    if torch.is_grad_enabled() and (y.requires_grad or (weight is not None and weight.requires_grad)):
+        return _CombineRows.apply(y, weight, groups)
+    return _combine(y, weight, groups)
 
 
 __all__ = ["RowGroups", "combine_rows", "group_rows"]
