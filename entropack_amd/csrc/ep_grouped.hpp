@@ -20,6 +20,18 @@ struct RowTile {
   int index;       // number of the tile within its group
 };
 
+// Sums of lanes 0 .. l, through the data-parallel lane moves (six dependent adds; the same scan through LDS takes ten times as long,
+// and every block of a product begins with one).
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);     // from 1 lane below, within rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);     // 2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);     // 4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);     // 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);     // lane 15 of a row to the next row: rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);     // lane 31 to rows 2 and 3
+  return v;
+}
+
 // Tile number `tile` of tiles of `tile_rows` places, in the order of the groups, those of no group last. Called by whole
 // waves; the result is the same in every lane.
 __device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ offsets, int groups, int entries, int tile, int tile_rows) {
@@ -33,12 +45,7 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ off
       high = offsets[g + 1];
     }
     const int n = (high - low + tile_rows - 1) / tile_rows;
-    int inclusive = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int other = __shfl_up(inclusive, d);
-      if (lane >= d) inclusive += other;
-    }
+    const int inclusive = wave_inclusive_sum(n);
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + inclusive > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
@@ -62,9 +69,7 @@ __device__ __forceinline__ int64_t count_row_tiles(const int32_t* __restrict__ o
   int mine = 0;
   for (int g = lane; g < groups; g += 64) mine += (offsets[g + 1] - offsets[g] + tile_rows - 1) / tile_rows;
   if (lane == 0) mine += (entries - offsets[groups] + tile_rows - 1) / tile_rows;
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
-  return __builtin_amdgcn_readfirstlane(mine);
+  return __builtin_amdgcn_readlane(wave_inclusive_sum(mine), 63);
 }
 
 // The most tiles of `tile_rows` places that `entries` places in `groups` groups (and the places of none) make.
@@ -163,13 +168,13 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
   if (kb < a.k_bytes) {                            // the last, partial piece: both operands are zero past the row's end
 #pragma unroll 1
     for (int s = 0; s < 4; ++s) {
-      uint4 fx[MT], fw[NT];
+      uint4 end_x[MT], end_w[NT];
       const bool inside = kb + 64 * s + piece < a.k_bytes;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) fx[t] = inside ? *reinterpret_cast<const uint4*>(from_x[t] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
+      for (int t = 0; t < MT; ++t) end_x[t] = inside ? *reinterpret_cast<const uint4*>(from_x[t] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fw[j] = inside ? *reinterpret_cast<const uint4*>(from_w[j] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
-      multiply(fx, fw);
+      for (int j = 0; j < NT; ++j) end_w[j] = inside ? *reinterpret_cast<const uint4*>(from_w[j] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
+      multiply(end_x, end_w);
     }
   }
   // Register i of lane l holds row 4 (l / 16) + i and column l % 16 of its 16 x 16 tile.

@@ -25,92 +25,176 @@ struct LowRankArgs {
 // 8 consecutive elements of a row of `up` from element e on; elements from `rank` on are zero. PIECES: rank, ldu and the
 // address allow 16-byte loads.
 template <bool PIECES>
-__device__ __forceinline__ bf16x8 up_piece(const uint16_t* __restrict__ row, int e, int rank) {
-  uint4 v = make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ uint4 up_piece(const uint16_t* __restrict__ row, int e, int rank) {
   if constexpr (PIECES) {
-    if (e < rank) v = *reinterpret_cast<const uint4*>(row + e);
+    // No branch around the load: one per load would serialise them.
+    const uint4 v = *reinterpret_cast<const uint4*>(row + (e < rank ? e : 0));
+    const uint32_t keep = e < rank ? ~0u : 0u;
+    return make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
   } else {
     uint32_t word[4] = {};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (e + i < rank) word[i >> 1] |= static_cast<uint32_t>(row[e + i]) << (16 * (i & 1));
-    v = make_uint4(word[0], word[1], word[2], word[3]);
+    return make_uint4(word[0], word[1], word[2], word[3]);
   }
-  return __builtin_bit_cast(bf16x8, v);
 }
 
-// A block takes 16 MT rows of one adapter and 256 columns, a wave 64 of them. The matrix cores are given the rows of `up` as
-// the left operand, ordered so that a lane ends up with 16 consecutive columns of its row (row m of tile j is column
-// 16 (m / 4) + 4 j + m % 4 of the wave's 64): y is read and out written 16 bytes at a time, 128 consecutive bytes per row, with no pass
-// through LDS. The inner dimension is [value | remainder], both against the same `up`.
-template <int MT, bool PIECES, bool WIDE>
+// Eight bf16 plus eight sums, each rounded once.
+__device__ __forceinline__ uint4 add_to_pieces(uint4 in, const f32x4& first, const f32x4& second) {
+  uint32_t word[4] = {in.x, in.y, in.z, in.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4& four = i < 2 ? first : second;
+    const float low = __uint_as_float(word[i] << 16) + four[2 * (i & 1)];
+    const float high = __uint_as_float(word[i] & 0xFFFF0000u) + four[2 * (i & 1) + 1];
+    word[i] = bf16_bits_of(low) | bf16_bits_of(high) << 16;
+  }
+  return make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+// Few rows per adapter: a block takes 16 rows of one adapter and 256 columns, a wave 64 of them. The matrix cores are given the rows
+// of `up` as the left operand, ordered so that a lane ends up with two runs of 8 consecutive columns of its row (row m of tile j
+// is column 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4 of the 64). The inner dimension is [value | remainder], both against the
+// same `up`. There is no LDS and nothing to wait for but the loads: 61 rows of 48 adapters take 3.5 us.
+template <bool PIECES, bool WIDE>
 __global__ __launch_bounds__(256) void low_rank_expand_kernel(LowRankArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int column_tiles = (a.N + 255) / 256;
-  const RowTile tile = find_row_tile(a.offsets, a.groups, a.entries, static_cast<int>(blockIdx.x / column_tiles), 16 * MT);
+  const RowTile tile = find_row_tile(a.offsets, a.groups, a.entries, static_cast<int>(blockIdx.x / column_tiles), 16);
   if (tile.group < 0) return;
   const int n0 = static_cast<int>(blockIdx.x % column_tiles) * 256 + wave * 64;
   if (n0 >= a.N) return;
   const int in_row = lane & 15, quarter = lane >> 4;
-  f32x4 acc[MT][4] = {};
+  const int at = in_row < tile.rows ? a.order[tile.first + in_row] : -1;
+  const int64_t to = at < a.rows ? at : -1;
+  const int n = n0 + 8 * quarter;
+  uint4 in[2];                                               // y is requested before anything else
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    in[h] = make_uint4(0, 0, 0, 0);
+    if (WIDE && a.y != nullptr && to >= 0 && n + 32 * h < a.N) in[h] = *reinterpret_cast<const uint4*>(a.y + to * a.ldy + n + 32 * h);
+  }
+  f32x4 acc[4] = {};
   if (tile.group < a.groups) {
+    const uint16_t* planes = a.planes + (static_cast<int64_t>(tile.first) + (in_row < tile.rows ? in_row : tile.rows - 1)) * (2 * a.padded) + 8 * quarter;
     const uint16_t* up[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int n = n0 + 16 * (in_row >> 2) + 4 * j + (in_row & 3);
-      up[j] = a.up + tile.group * a.up_group + (n < a.N ? n : a.N - 1) * a.ldu;
-    }
-    const uint16_t* planes[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int row = 16 * t + in_row;
-      planes[t] = a.planes + (static_cast<int64_t>(tile.first) + (row < tile.rows ? row : tile.rows - 1)) * (2 * a.padded) + 8 * quarter;
+      const int row = n0 + 32 * (j >> 1) + 8 * (in_row >> 2) + 4 * (j & 1) + (in_row & 3);
+      up[j] = a.up + tile.group * a.up_group + (row < a.N ? row : a.N - 1) * a.ldu;
     }
     for (int e0 = 0; e0 < 2 * a.padded; e0 += 32) {
-      bf16x8 fp[MT];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) fp[t] = *reinterpret_cast<const bf16x8*>(planes[t] + e0);
       const int e = e0 + 8 * quarter, in_up = e < a.padded ? e : e - a.padded;
+      const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + e0);
+      bf16x8 fu[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bf16x8 fu = up_piece<PIECES>(up[j], in_up, a.rank);
+      for (int j = 0; j < 4; ++j) fu[j] = __builtin_bit_cast(bf16x8, up_piece<PIECES>(up[j], in_up, a.rank));
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fu, fp[t], acc[t][j], 0, 0, 0);
+      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fu[j], fp, acc[j], 0, 0, 0);
+    }
+  }
+  if (to < 0) return;
+  // Column n + 32 (j / 2) + 4 (j % 2) + i is in register i of tile j.
+  uint16_t* out = a.out + to * a.ldo + n;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (n + 32 * h >= a.N) continue;
+      *reinterpret_cast<uint4*>(out + 32 * h) = add_to_pieces(in[h], acc[2 * h], acc[2 * h + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const int column = 32 * (c >> 3) + (c & 7);
+      if (n + column >= a.N) continue;
+      const float v = a.y != nullptr ? __uint_as_float(static_cast<uint32_t>(a.y[to * a.ldy + n + column]) << 16) : 0.0f;
+      out[column] = static_cast<uint16_t>(bf16_bits_of(v + acc[c >> 2][c & 3]));
+    }
+  }
+}
+
+// Many rows per adapter: bound by reading y and writing out. A block takes 64 rows of one adapter, 16 per wave, and 128 columns.
+// Memory wants neighbouring lanes at neighbouring addresses (a load whose lanes are on sixteen rows, as the fragments of the kernel
+// above are, occupies the address path four times as long: 7993 rows of 4096, rank 32, 46 us with it). So `up` goes through LDS,
+// STEP ranks at a time, fetched once for all 64 rows, and the planes are the left operand: lane l then holds, over the eight
+// 16-column tiles (row m of tile j is column 8 m + j), 8 consecutive columns 8 (l % 16) .. of rows 4 (l / 16) + i: sixteen lanes
+// read and write 256 consecutive bytes of a row. Small blocks, so that many are resident and the last round is short: 34 us
+// (256 columns per block 41, 512 columns 44; a copy of the same bytes 21).
+// STEP: the least of 16, 32 and 64 that the rank fits, 64 beyond.
+constexpr int kTallColumns = 128;
+
+template <bool PIECES, bool WIDE, int STEP>
+__global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a) {
+  constexpr int kPieces = STEP / 8, kMoves = kTallColumns * kPieces / 256;
+  constexpr int kPitch = STEP * 2 + 16;                      // bytes per column of `up`: an odd number of 16-byte pieces, all banks
+  __shared__ __align__(16) uint8_t up_tile[kTallColumns * kPitch];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int column_tiles = (a.N + kTallColumns - 1) / kTallColumns;
+  const RowTile tile = find_row_tile(a.offsets, a.groups, a.entries, static_cast<int>(blockIdx.x / column_tiles), 64);
+  if (tile.group < 0) return;
+  const int first_column = static_cast<int>(blockIdx.x % column_tiles) * kTallColumns;
+  const int in_row = lane & 15, quarter = lane >> 4, n = first_column + 8 * in_row;
+  const bool grouped = tile.group < a.groups;
+  int64_t to[4];                                             // rows 16 wave + 4 quarter + i
+  uint4 in[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 16 * wave + 4 * quarter + i;
+    const int at = row < tile.rows ? a.order[tile.first + row] : -1;
+    to[i] = at < a.rows ? at : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    in[i] = make_uint4(0, 0, 0, 0);
+    if (WIDE && a.y != nullptr && to[i] >= 0 && n < a.N) in[i] = *reinterpret_cast<const uint4*>(a.y + to[i] * a.ldy + n);
+  }
+  f32x4 acc[8] = {};
+  if (grouped) {
+    const int plane_row = 16 * wave + in_row < tile.rows ? 16 * wave + in_row : tile.rows - 1;
+    const uint16_t* planes = a.planes + (static_cast<int64_t>(tile.first) + plane_row) * (2 * a.padded) + (quarter >> 1) * a.padded;
+    const uint16_t* up = a.up + tile.group * a.up_group;
+    for (int rank0 = 0; rank0 < a.padded; rank0 += STEP) {
+      uint4 moved[kMoves];
+#pragma unroll
+      for (int m = 0; m < kMoves; ++m) {
+        const int cell = tid + 256 * m, column = first_column + cell / kPieces;
+        moved[m] = up_piece<PIECES>(up + (column < a.N ? column : a.N - 1) * a.ldu, rank0 + 8 * (cell % kPieces), a.rank);
+      }
+      if (rank0 > 0) __syncthreads();                        // the stretch before has been read
+#pragma unroll
+      for (int m = 0; m < kMoves; ++m) {
+        const int cell = tid + 256 * m, column = cell / kPieces;                  // column 8 m + j lies at 16 j + m
+        *reinterpret_cast<uint4*>(up_tile + ((column & 7) * 16 + (column >> 3)) * kPitch + 16 * (cell % kPieces)) = moved[m];
+      }
+      __syncthreads();
+      const int ranks = a.padded - rank0 < STEP ? a.padded - rank0 : STEP;
+      // 32 of the inner dimension at a time: 16 ranks' values and remainders (quarters 0, 1 and 2, 3), both against the same `up`.
+      for (int e0 = 0; e0 < ranks; e0 += 16) {
+        const int e = e0 + 8 * (quarter & 1);
+        const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + rank0 + e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bf16x8 fu = *reinterpret_cast<const bf16x8*>(up_tile + (16 * j + in_row) * kPitch + 2 * e);
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp, fu, acc[j], 0, 0, 0);
+        }
       }
     }
   }
-  // Lane (row in_row, quarter): columns n0 + 16 quarter + 4 j + i in register i of tile j.
+  // Row 4 quarter + i, column n + j is in register i of tile j.
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int row = 16 * t + in_row;
-    if (row >= tile.rows) continue;
-    int to = a.order[tile.first + row];
-    if (to >= a.rows) continue;
-    const int n = n0 + 16 * quarter;
-    const uint16_t* from = a.y != nullptr ? a.y + to * a.ldy + n : nullptr;
-    uint16_t* out = a.out + to * a.ldo + n;
+  for (int i = 0; i < 4; ++i) {
+    if (to[i] < 0) continue;
+    uint16_t* out = a.out + to[i] * a.ldo + n;
+    const f32x4 low = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]}, high = {acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
     if constexpr (WIDE) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (n + 8 * h >= a.N) continue;
-        uint4 in = make_uint4(0, 0, 0, 0);
-        if (from != nullptr) in = *reinterpret_cast<const uint4*>(from + 8 * h);
-        uint32_t word[4] = {in.x, in.y, in.z, in.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4& four = acc[t][2 * h + (i >> 1)];
-          const float low = __uint_as_float(word[i] << 16) + four[2 * (i & 1)];
-          const float high = __uint_as_float(word[i] & 0xFFFF0000u) + four[2 * (i & 1) + 1];
-          word[i] = bf16_bits_of(low) | bf16_bits_of(high) << 16;
-        }
-        *reinterpret_cast<uint4*>(out + 8 * h) = make_uint4(word[0], word[1], word[2], word[3]);
-      }
+      if (n < a.N) *reinterpret_cast<uint4*>(out) = add_to_pieces(in[i], low, high);
     } else {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        if (n + c >= a.N) continue;
-        const float v = from != nullptr ? __uint_as_float(static_cast<uint32_t>(from[c]) << 16) : 0.0f;
-        out[c] = static_cast<uint16_t>(bf16_bits_of(v + acc[t][c >> 2][c & 3]));
+      for (int j = 0; j < 8; ++j) {
+        if (n + j >= a.N) continue;
+        const float v = a.y != nullptr ? __uint_as_float(static_cast<uint32_t>(a.y[to[i] * a.ldy + n + j]) << 16) : 0.0f;
+        out[j] = static_cast<uint16_t>(bf16_bits_of(v + (j < 4 ? low[j & 3] : high[j & 3])));
       }
     }
   }
@@ -197,7 +281,10 @@ int ep_hip_low_rank_shrink(const void* x_dev, int64_t ldx, const void* down_dev,
   a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(down_dev), a.scale_x = scale_dev, a.y = planes_dev, a.row_of = order_dev, a.offsets = offsets_dev;
   a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = (rank + 15) / 16 * 16 * 2;
   a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(entries), a.out_kind = kOutBF16;
-  return launch_stream_of<false, 1, 1, 4, true>(a, static_cast<hipStream_t>(stream));
+  // 32 rows and all of a small rank per block, so that x is read once and `down` half as often as with 16 rows: 7993 rows of 4096, rank
+  // 32, 22.6 us (16 rows and 32 ranks 27.0, 16 and 16 32.4); few rows take the same time in every shape.
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return rank <= 16 ? launch_stream_of<false, 2, 1, 8, true>(a, s) : launch_stream_of<false, 2, 2, 8, true>(a, s);
 }
 
 int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t ldu, int64_t up_group, const void* y_dev, int64_t ldy, void* out_dev, int64_t ldo,
@@ -214,14 +301,27 @@ int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t l
   auto in_pieces = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
   const bool pieces = in_pieces(up_dev, ldu) && up_group % 8 == 0 && rank % 8 == 0;
   const bool wide = in_pieces(out_dev, ldo) && N % 8 == 0 && (y_dev == nullptr || in_pieces(y_dev, ldy));
-  const int64_t blocks = most_row_tiles(entries, groups, 16) * ((N + 255) / 256);
+  const bool tall = entries / groups >= 32;                  // most blocks of 64 rows are then at least half full
+  const int columns = tall ? kTallColumns : 256;
+  const int64_t blocks = most_row_tiles(entries, groups, tall ? 64 : 16) * ((N + columns - 1) / columns);
   if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (pieces && wide) hipLaunchKernelGGL((low_rank_expand_kernel<1, true, true>), grid, dim3(256), 0, s, a);
-  else if (pieces) hipLaunchKernelGGL((low_rank_expand_kernel<1, true, false>), grid, dim3(256), 0, s, a);
-  else if (wide) hipLaunchKernelGGL((low_rank_expand_kernel<1, false, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((low_rank_expand_kernel<1, false, false>), grid, dim3(256), 0, s, a);
+#define EP_EXPAND(PIECES, WIDE)                                                                                               \
+  if (!tall) hipLaunchKernelGGL((low_rank_expand_kernel<PIECES, WIDE>), grid, dim3(256), 0, s, a);                             \
+  else if (a.padded <= 16) hipLaunchKernelGGL((low_rank_expand_tall_kernel<PIECES, WIDE, 16>), grid, dim3(256), 0, s, a);      \
+  else if (a.padded <= 32) hipLaunchKernelGGL((low_rank_expand_tall_kernel<PIECES, WIDE, 32>), grid, dim3(256), 0, s, a);      \
+  else hipLaunchKernelGGL((low_rank_expand_tall_kernel<PIECES, WIDE, 64>), grid, dim3(256), 0, s, a)
+  if (pieces && wide) {
+    EP_EXPAND(true, true);
+  } else if (pieces) {
+    EP_EXPAND(true, false);
+  } else if (wide) {
+    EP_EXPAND(false, true);
+  } else {
+    EP_EXPAND(false, false);
+  }
+#undef EP_EXPAND
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
 }
