@@ -74,13 +74,15 @@ static int tile_for(int64_t entries, int groups, int64_t columns) {
 
 template <bool INT8>
 static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
-  // Few rows per group: the weights' stream (MI355X, weights from memory). One row per group or so, blocks of 16 weight rows: one token,
-  // two of eight experts 4096 x 4096, 14.1 us (32 weight rows 16.2; floor 10.2); 18 tokens, four of 64 experts 1408 x 2048,
-  // 36.9 us. From five rows on 32 rows by 64 weight rows: 64 tokens, two of eight, 71 us (16 x 32: 80; 128 x 128 tiles 90).
-  // From 32 rows on the 128 x 128 tiles: 512 tokens, four of 64, 104 us against 112; 256 tokens, two of eight, 84 against 115.
+  // Few rows per group: the weights' stream (MI355X, weights from memory). About one row per group: blocks of 16 weight rows; one token,
+  // two of eight experts 4096 x 4096, 12.7 us (floor 10.2), 18 tokens, four of 64 experts 1408 x 2048, 31.1 us. From five rows on
+  // 32 rows by 32 weight rows (64 tokens, two of eight, 62 us; 256 tokens, four of 64, 75), from 24 on by 64 (128 tokens, two of
+  // eight, 61 us against 73; 512 tokens, four of 64, 98 against 96). From 48 on the 128 x 128 tiles: 256 tokens, two of eight, 82 us
+  // against 91; 1024 tokens, four of 64, 106 against 135.
   const int mean = a.entries / a.groups;
-  if (mean < 5) return launch_stream_of<INT8, 1, 1, 8, false>(a, s);
-  if (mean < 32) return launch_stream_of<INT8, 2, 4, 8, false>(a, s);
+  if (mean < 5) return launch_stream_of<INT8, 1, 1, 4, false>(a, s);
+  if (mean < 24) return launch_stream_of<INT8, 2, 2, 2, false>(a, s);
+  if (mean < 48) return launch_stream_of<INT8, 2, 4, 2, false>(a, s);
   TileArgs t = {};
   t.a = a.x, t.b = a.w, t.scale_x = a.scale_x, t.scale_w = a.scale_w, t.bias = a.bias, t.y = a.y, t.row_of = a.row_of, t.offsets = a.offsets;
   t.lda_bytes = a.ldx_bytes, t.ldb_bytes = a.ldw_bytes, t.group_b_bytes = a.group_bytes, t.ldy = a.ldy;

@@ -13,6 +13,17 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int64_t kMostEntries = int64_t{1} << 30;
 
+// What a lane loads whose piece lies past an operand's end.
+__device__ __align__(16) const uint32_t kZeroPiece[4] = {0, 0, 0, 0};
+
+// 16 bytes of global memory. (An address chosen between an operand and the zeros has no address space of its own, and a load that
+// might be one of LDS waits for every LDS access.)
+__device__ __forceinline__ uint4 load_piece(const uint8_t* from) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 v = *(const __attribute__((address_space(1))) u32x4*)from;
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 struct RowTile {
   int group;       // `groups` for a tile of rows without a group, -1 past the last tile
   int first;       // first place of the tile
@@ -100,10 +111,11 @@ __device__ __forceinline__ int source_row(const GroupedArgs& a, int place) {
 
 // ---- few rows per group: the weight's stream bounds the product -------------------------------------------------------------
 //
-// A block takes 16 MT rows and 16 NT weight rows; its waves take every WAVES-th piece of 256 bytes of K and the sums meet in
-// LDS. Both operands go from memory straight into the fragments of the 16 x 16 matrix-core instructions (lane l holds 16
-// bytes of row l % 16 at byte 16 (l / 16) of a 64-byte step: 64 consecutive bytes per row and instruction), so there is no
-// barrier in the loop and every wave keeps 4 (MT + NT) loads of 1 KiB in flight.
+// A block takes 16 MT rows and 16 NT weight rows; its waves take every WAVES-th piece of 256 bytes of K, each by itself, and the
+// sums meet in LDS. Memory wants neighbouring lanes at neighbouring addresses: a load takes 256 bytes of each of four rows. The
+// fragments of the 16 x 16 matrix-core instructions want sixteen rows (lane l holds 16 bytes of row l % 16, at byte 16 (l / 16)
+// of a 64-byte step): the piece goes through LDS private to the wave, while the next one is on its way in registers, so that
+// there is no barrier in the loop. Loading the fragments straight from memory occupies the address path four times as long.
 // PLANES: the sums are multiplied with scale_x[group] and stored as two bf16 parts, the rounded value and the rounded
 // remainder, columns [0, padded) and [padded, 2 padded) of row p of y, padded = N rounded up to 16; columns from N on are 0.
 // The product that reads them then works on 16 bits of significand instead of 8, in the memory that f32 would take.
@@ -113,7 +125,10 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
   using Frag = typename std::conditional<INT8, i32x4, bf16x8>::type;
   using Cell = typename std::conditional<INT8, int32_t, float>::type;
   constexpr int kRows = 16 * MT, kColumns = 16 * NT, kPitch = kColumns + 4;
-  __shared__ __align__(16) Cell sums[WAVES][kRows][kPitch];
+  constexpr int kStagedPitch = 256 + 16;           // bytes of a staged row: an odd number of 16-byte pieces, all banks
+  constexpr int kStagedBytes = 16 * (MT + NT) * kStagedPitch, kSumsBytes = kRows * kPitch * 4;       // of a wave
+  __shared__ __align__(16) uint8_t room[WAVES * (kStagedBytes > kSumsBytes ? kStagedBytes : kSumsBytes)];
+  Cell(*sums)[kRows][kPitch] = reinterpret_cast<Cell(*)[kRows][kPitch]>(room);                       // once every wave is done with its stage
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column_tiles = (a.N + kColumns - 1) / kColumns;
@@ -129,54 +144,59 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
     }
     return;
   }
-  const int in_row = lane & 15, piece = (lane >> 4) * 16;
-  const uint8_t* from_x[MT];
-  const uint8_t* from_w[NT];
+  uint8_t* const staged = room + wave * kStagedBytes;
+  auto staged_at = [&](int row, int byte) { return staged + row * kStagedPitch + byte; };
+  const int in_row = lane & 15;
+  const int load_row = lane >> 4, load_at = 16 * (lane & 15);         // row 4 i + load_row of load i, its bytes
+  const uint8_t* from_x[4 * MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int row = 16 * t + in_row;
-    from_x[t] = a.x + source_row(a, tile.first + (row < tile.rows ? row : tile.rows - 1)) * a.ldx_bytes + piece;
+  for (int i = 0; i < 4 * MT; ++i) {
+    const int row = 4 * i + load_row;
+    from_x[i] = a.x + source_row(a, tile.first + (row < tile.rows ? row : tile.rows - 1)) * a.ldx_bytes + load_at;
   }
+  const uint8_t* from_w[4 * NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int n = n0 + 16 * j + in_row;
-    from_w[j] = a.w + tile.group * a.group_bytes + (n < a.N ? n : a.N - 1) * a.ldw_bytes + piece;
+  for (int i = 0; i < 4 * NT; ++i) {
+    const int n = n0 + 4 * i + load_row;
+    from_w[i] = a.w + tile.group * a.group_bytes + (n < a.N ? n : a.N - 1) * a.ldw_bytes + load_at;
   }
+  const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeroPiece);
   Acc acc[MT][NT] = {};
-  auto multiply = [&](const uint4 (&fx)[MT], const uint4 (&fw)[NT]) {
+  uint4 held_x[4 * MT], held_w[4 * NT];
+  auto fetch = [&](int64_t kb) {                   // both operands are zero past the row's end
+    const bool inside = kb + load_at < a.k_bytes;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int i = 0; i < 4 * NT; ++i) held_w[i] = load_piece(inside ? from_w[i] + kb : zeros);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if constexpr (INT8) acc[t][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(Frag, fx[t]), __builtin_bit_cast(Frag, fw[j]), acc[t][j], 0, 0, 0);
-        else acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Frag, fx[t]), __builtin_bit_cast(Frag, fw[j]), acc[t][j], 0, 0, 0);
-      }
+    for (int i = 0; i < 4 * MT; ++i) held_x[i] = load_piece(inside ? from_x[i] + kb : zeros);
   };
-  int64_t kb = wave * 256;
-  for (; kb + 256 <= a.k_bytes; kb += WAVES * 256) {
-    uint4 fx[4][MT], fw[4][NT];
+  const int64_t stride = WAVES * 256;
+  if (wave * 256 < a.k_bytes) fetch(wave * 256);
+  for (int64_t kb = wave * 256; kb < a.k_bytes; kb += stride) {
+#pragma unroll
+    for (int i = 0; i < 4 * MT; ++i) *reinterpret_cast<uint4*>(staged_at(4 * i + load_row, load_at)) = held_x[i];
+#pragma unroll
+    for (int i = 0; i < 4 * NT; ++i) *reinterpret_cast<uint4*>(staged_at(16 * MT + 4 * i + load_row, load_at)) = held_w[i];
+    if (kb + stride < a.k_bytes) fetch(kb + stride);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
+      Frag fx[MT], fw[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fw[s][j] = *reinterpret_cast<const uint4*>(from_w[j] + kb + 64 * s);
+      for (int t = 0; t < MT; ++t) fx[t] = *reinterpret_cast<const Frag*>(staged_at(16 * t + in_row, 64 * s + 16 * (lane >> 4)));
 #pragma unroll
-      for (int t = 0; t < MT; ++t) fx[s][t] = *reinterpret_cast<const uint4*>(from_x[t] + kb + 64 * s);
+      for (int j = 0; j < NT; ++j) fw[j] = *reinterpret_cast<const Frag*>(staged_at(16 * (MT + j) + in_row, 64 * s + 16 * (lane >> 4)));
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if constexpr (INT8) acc[t][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fx[t], fw[j], acc[t][j], 0, 0, 0);
+          else acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[t], fw[j], acc[t][j], 0, 0, 0);
+        }
     }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) multiply(fx[s], fw[s]);
+    __builtin_amdgcn_wave_barrier();
   }
-  if (kb < a.k_bytes) {                            // the last, partial piece: both operands are zero past the row's end
-#pragma unroll 1
-    for (int s = 0; s < 4; ++s) {
-      uint4 end_x[MT], end_w[NT];
-      const bool inside = kb + 64 * s + piece < a.k_bytes;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) end_x[t] = inside ? *reinterpret_cast<const uint4*>(from_x[t] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) end_w[j] = inside ? *reinterpret_cast<const uint4*>(from_w[j] + kb + 64 * s) : make_uint4(0, 0, 0, 0);
-      multiply(end_x, end_w);
-    }
-  }
+  __syncthreads();
   // Register i of lane l holds row 4 (l / 16) + i and column l % 16 of its 16 x 16 tile.
 #pragma unroll
   for (int t = 0; t < MT; ++t)

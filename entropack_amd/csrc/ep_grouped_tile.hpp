@@ -26,8 +26,6 @@
 
 namespace ep {
 
-__device__ __align__(16) const uint32_t kZeroPiece[4] = {0, 0, 0, 0};
-
 struct TileArgs {
   const uint8_t* a;                // left operand
   const uint8_t* b;                // right operand

@@ -281,10 +281,12 @@ int ep_hip_low_rank_shrink(const void* x_dev, int64_t ldx, const void* down_dev,
   a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(down_dev), a.scale_x = scale_dev, a.y = planes_dev, a.row_of = order_dev, a.offsets = offsets_dev;
   a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = (rank + 15) / 16 * 16 * 2;
   a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(entries), a.out_kind = kOutBF16;
-  // 32 rows and all of a small rank per block, so that x is read once and `down` half as often as with 16 rows: 7993 rows of 4096, rank
-  // 32, 22.6 us (16 rows and 32 ranks 27.0, 16 and 16 32.4); few rows take the same time in every shape.
+  // All of a rank up to 64 in one block, so that x is read once. 4099 rows of 4096: rank 16 9.0 us (8 waves 10.5; 500 rows 6.0 against
+  // 5.4), rank 64 16.1 us (32 ranks per block 19.2); 7993 rows, rank 32, 18.5 us (16 rows per block 19.6; reading x takes 10.6).
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return rank <= 16 ? launch_stream_of<false, 2, 1, 8, true>(a, s) : launch_stream_of<false, 2, 2, 8, true>(a, s);
+  if (rank > 32) return launch_stream_of<false, 2, 4, 4, true>(a, s);
+  if (rank > 16) return launch_stream_of<false, 2, 2, 8, true>(a, s);
+  return entries >= 2048 ? launch_stream_of<false, 1, 1, 4, true>(a, s) : launch_stream_of<false, 1, 1, 8, true>(a, s);
 }
 
 int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t ldu, int64_t up_group, const void* y_dev, int64_t ldy, void* out_dev, int64_t ldo,
