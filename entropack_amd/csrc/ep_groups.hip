@@ -29,23 +29,52 @@ __device__ __forceinline__ uint64_t lanes_with_my_key(int key, int key_bits, uin
   return same;
 }
 
-// counts[wave][key] (LDS, row stride groups + 1, cleared before) += this wave's entries [first, last).
+// LDS accesses before it, of any lane of this wave, come before those after it.
+__device__ __forceinline__ void order_in_wave() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// counts[key] (LDS, this wave's row, cleared before) += this wave's entries [first, last).
 template <typename Id>
 __device__ __forceinline__ void count_entries(const Id* __restrict__ ids, int64_t first, int64_t last, int groups, int key_bits, int* counts) {
   const int lane = threadIdx.x & 63;
-  for (int64_t at = first; at < last; at += 64) {
-    const bool live = at + lane < last;
-    const int key = live ? group_of(ids, at + lane, groups) : 0;
-    const uint64_t same = lanes_with_my_key(key, key_bits, __builtin_amdgcn_ballot_w64(live));
-    if (live && __builtin_ctzll(same) == lane) counts[key] += __builtin_popcountll(same);
-    __builtin_amdgcn_wave_barrier();           // LDS accesses of a wave keep their order
+  constexpr int kTogether = 4;                   // loads under way at a time; those past the end read the last id
+  for (int64_t from = first; from < last; from += 64 * kTogether) {
+    int key[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int64_t at = from + 64 * i + lane;
+      key[i] = group_of(ids, at < last ? at : last - 1, groups);
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const bool live = from + 64 * i + lane < last;
+      const uint64_t same = lanes_with_my_key(key[i], key_bits, __builtin_amdgcn_ballot_w64(live));
+      if (live && __builtin_ctzll(same) == lane) counts[key[i]] += __builtin_popcountll(same);
+      order_in_wave();
+    }
   }
 }
 
+// What the sort writes.
+struct GroupOut {
+  int32_t* order;
+  int32_t* offsets;
+  int32_t* place;
+  int32_t* rows;                   // may be absent
+  int per_row;
+
+  __device__ __forceinline__ void put(int64_t entry, int to) const {
+    order[to] = static_cast<int32_t>(entry);
+    place[entry] = to;
+    if (rows != nullptr) rows[to] = static_cast<int32_t>(static_cast<uint32_t>(entry) / static_cast<uint32_t>(per_row));
+  }
+};
+
 // Gives every entry its place; next[key] (LDS, this wave's row) is the place of the wave's next entry with that key.
 template <typename Id>
-__device__ __forceinline__ void place_entries(const Id* __restrict__ ids, int64_t first, int64_t last, int groups, int key_bits, int* next,
-                                              int per_row, int32_t* __restrict__ order, int32_t* __restrict__ place, int32_t* __restrict__ rows) {
+__device__ __forceinline__ void place_entries(const Id* __restrict__ ids, int64_t first, int64_t last, int groups, int key_bits, int* next, const GroupOut& out) {
   const int lane = threadIdx.x & 63;
   for (int64_t at = first; at < last; at += 64) {
     const bool live = at + lane < last;
@@ -53,14 +82,11 @@ __device__ __forceinline__ void place_entries(const Id* __restrict__ ids, int64_
     const uint64_t same = lanes_with_my_key(key, key_bits, __builtin_amdgcn_ballot_w64(live));
     if (live) {
       const int base = next[key];
-      const int to = base + __builtin_popcountll(same & ((uint64_t{1} << lane) - 1));
-      order[to] = static_cast<int32_t>(at + lane);
-      place[at + lane] = to;
-      if (rows != nullptr) rows[to] = static_cast<int32_t>(static_cast<uint32_t>(at + lane) / static_cast<uint32_t>(per_row));
-      __builtin_amdgcn_wave_barrier();           // the leader moves the row on once every lane of the wave has read it
+      out.put(at + lane, base + __builtin_popcountll(same & ((uint64_t{1} << lane) - 1)));
+      order_in_wave();                           // the leader moves the row on once every lane of the wave has read it
       if (__builtin_ctzll(same) == lane) next[key] = base + __builtin_popcountll(same);
     }
-    __builtin_amdgcn_wave_barrier();
+    order_in_wave();
   }
 }
 
@@ -86,33 +112,49 @@ __global__ __launch_bounds__(kGroupThreads) void group_count_kernel(const Id* __
   }
 }
 
-// Places this block's entries. The counts of all blocks come from `table`; a single block (table == nullptr) needs none.
-// LDS: per-wave rows [kGroupWaves][keys], then before[keys] (entries of a key in earlier blocks) and total[keys].
-template <typename Id>
+// Places this block's entries. What the other blocks hold of each key comes from `table`; a single block needs none.
+// LDS: per-wave rows [kGroupWaves][keys], then before[keys] (entries of a key in earlier blocks) and others[keys] (in all
+// other blocks). PER > 0: a block has 64 PER kGroupWaves entries, whose ranks stay in registers from the count to the
+// placing; PER == 0: any number, which are read and ranked again.
+template <typename Id, int PER>
 __global__ __launch_bounds__(kGroupThreads) void group_place_kernel(const Id* __restrict__ ids, int64_t entries, int64_t chunk, int groups,
-                                                                    int key_bits, const int32_t* __restrict__ table, int blocks, int per_row,
-                                                                    int32_t* __restrict__ order, int32_t* __restrict__ offsets,
-                                                                    int32_t* __restrict__ place, int32_t* __restrict__ rows) {
+                                                                    int key_bits, const int32_t* __restrict__ table, int blocks, GroupOut out) {
   extern __shared__ int group_smem[];
   __shared__ int wave_sums[kGroupWaves];
   const int keys = groups + 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* counts = group_smem + wave * keys;
   int* before = group_smem + kGroupWaves * keys;
-  int* total = before + keys;
+  int* others = before + keys;
+  const int64_t begin = blockIdx.x * chunk, end = begin + chunk < entries ? begin + chunk : entries;
+  const int64_t share = PER > 0 ? PER * 64 : ((end - begin + kGroupWaves * 64 - 1) / (kGroupWaves * 64)) * 64;
+  const int64_t first = begin + wave * share, last = first + share < end ? first + share : end;
+  int mine_key[PER > 0 ? PER : 1], rank[PER > 0 ? PER : 1];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine_key[i] = first + 64 * i + lane < last ? group_of(ids, first + 64 * i + lane, groups) : 0;
   for (int i = threadIdx.x; i < (kGroupWaves + 2) * keys; i += kGroupThreads) group_smem[i] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t begin = blockIdx.x * chunk, end = begin + chunk < entries ? begin + chunk : entries;
-  const int64_t share = ((end - begin + kGroupWaves * 64 - 1) / (kGroupWaves * 64)) * 64;
-  const int64_t first = begin + wave * share, last = first + share < end ? first + share : end;
-  count_entries(ids, first, last, groups, key_bits, group_smem + wave * keys);
+  if constexpr (PER == 0) {
+    count_entries(ids, first, last, groups, key_bits, counts);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool live = first + 64 * i + lane < last;
+      const uint64_t same = lanes_with_my_key(mine_key[i], key_bits, __builtin_amdgcn_ballot_w64(live));
+      const int seen = live ? counts[mine_key[i]] : 0;
+      rank[i] = seen + __builtin_popcountll(same & ((uint64_t{1} << lane) - 1));
+      order_in_wave();                           // the leader moves the row on once every lane of the wave has read it
+      if (live && __builtin_ctzll(same) == lane) counts[mine_key[i]] = seen + __builtin_popcountll(same);
+      order_in_wave();
+    }
+  }
   if (table != nullptr) {
     const int cells = blocks * keys;             // integer sums: their order does not matter
     for (int i = threadIdx.x; i < cells; i += kGroupThreads) {
-      const int n = table[i];
-      if (n != 0) {
-        const int key = i % keys;
-        atomicAdd(&total[key], n);
-        if (i / keys < static_cast<int>(blockIdx.x)) atomicAdd(&before[key], n);
+      const int n = table[i], block = i / keys, key = i % keys;
+      if (n != 0 && block != static_cast<int>(blockIdx.x)) {
+        atomicAdd(&others[key], n);
+        if (block < static_cast<int>(blockIdx.x)) atomicAdd(&before[key], n);
       }
     }
   }
@@ -121,25 +163,17 @@ __global__ __launch_bounds__(kGroupThreads) void group_place_kernel(const Id* __
   const int key = threadIdx.x;
   int mine = 0;
   if (key < keys) {
-    if (table != nullptr) {
-      mine = total[key];
-    } else {
+    mine = others[key];
 #pragma unroll
-      for (int w = 0; w < kGroupWaves; ++w) mine += group_smem[w * keys + key];
-    }
+    for (int w = 0; w < kGroupWaves; ++w) mine += group_smem[w * keys + key];
   }
-  int inclusive = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int other = __shfl_up(inclusive, d);
-    if (lane >= d) inclusive += other;
-  }
+  const int inclusive = wave_inclusive_sum(mine);
   if (lane == 63) wave_sums[wave] = inclusive;
   __syncthreads();
   int start = inclusive - mine;
   for (int w = 0; w < wave; ++w) start += wave_sums[w];
   if (key < keys) {
-    if (blockIdx.x == 0) offsets[key] = start;           // offsets[groups]: entries that have a group
+    if (blockIdx.x == 0) out.offsets[key] = start;           // offsets[groups]: entries that have a group
     int at = start + before[key];
 #pragma unroll
     for (int w = 0; w < kGroupWaves; ++w) {
@@ -149,33 +183,53 @@ __global__ __launch_bounds__(kGroupThreads) void group_place_kernel(const Id* __
     }
   }
   __syncthreads();
-  place_entries(ids, first, last, groups, key_bits, group_smem + wave * keys, per_row, order, place, rows);
+  if constexpr (PER == 0) {
+    place_entries(ids, first, last, groups, key_bits, counts, out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (first + 64 * i + lane < last) out.put(first + 64 * i + lane, counts[mine_key[i]] + rank[i]);
+    }
+  }
 }
 
-// Entries one block sorts before another block takes the rest, and the most blocks.
-constexpr int64_t kGroupChunk = 4096;
+// One block sorts up to kOneBlock entries; beyond, a kernel before it counts blocks of 4096, and more than kGroupBlocks of
+// those give each block a longer share. In 16 and 256 groups, one block: 1000 entries 3.2 and 3.7 us, 4096 5.7 and 7.4 us,
+// 8192 9.0 and 12.4 us; two kernels: 4096 9.1 and 11.6 us, 8192 9.3 and 12.1 us besides a second launch, 16384 10.1 and
+// 13.0 us, 131072 11.0 and 16.8 us. Latency bounds all of these (131072 ids of 64 bits and what is written of them, 2.6 MB,
+// are 0.4 us); every block counting the others' ids by itself in place of the first kernel took 12.0 us for 16384 entries.
+constexpr int64_t kOneBlock = 8 * kGroupThreads;
+constexpr int64_t kGroupChunk = 4 * kGroupThreads;
 constexpr int kGroupBlocks = 256;
 constexpr int kMostGroups = 896;                 // a thread per key in the scan, 64 KiB of LDS
 
 static int64_t group_chunk(int64_t entries) {
+  if (entries <= kOneBlock) return entries <= kGroupThreads ? kGroupThreads : entries <= kGroupChunk ? kGroupChunk : kOneBlock;
   const int64_t even = (entries + kGroupBlocks - 1) / kGroupBlocks;
   return even < kGroupChunk ? kGroupChunk : (even + 63) / 64 * 64;
 }
 
 template <typename Id>
-static int launch_group(const Id* ids, int64_t entries, int groups, int per_row, int32_t* order, int32_t* offsets, int32_t* place, int32_t* rows, int32_t* table,
-                        hipStream_t s) {
+static int launch_group(const Id* ids, int64_t entries, int groups, const GroupOut& out, int32_t* table, hipStream_t s) {
   const int64_t chunk = group_chunk(entries);
   const int blocks = static_cast<int>((entries + chunk - 1) / chunk);
   const int keys = groups + 1;
+  const size_t room = (kGroupWaves + 2) * keys * sizeof(int);
   int key_bits = 0;
   while ((groups >> key_bits) != 0) ++key_bits;
-  if (blocks > 1) {
-    hipLaunchKernelGGL(group_count_kernel<Id>, dim3(blocks), dim3(kGroupThreads), kGroupWaves * keys * sizeof(int), s, ids, entries, chunk, groups, key_bits, table);
+  if (entries <= kOneBlock) {
+    if (chunk == kGroupThreads) hipLaunchKernelGGL((group_place_kernel<Id, 1>), dim3(1), dim3(kGroupThreads), room, s, ids, entries, chunk, groups, key_bits, nullptr, 1, out);
+    else if (chunk == kGroupChunk) hipLaunchKernelGGL((group_place_kernel<Id, 4>), dim3(1), dim3(kGroupThreads), room, s, ids, entries, chunk, groups, key_bits, nullptr, 1, out);
+    else hipLaunchKernelGGL((group_place_kernel<Id, 8>), dim3(1), dim3(kGroupThreads), room, s, ids, entries, chunk, groups, key_bits, nullptr, 1, out);
     EP_HIP_TRY(hipGetLastError());
+    return EP_HIP_OK;
   }
-  hipLaunchKernelGGL(group_place_kernel<Id>, dim3(blocks), dim3(kGroupThreads), (kGroupWaves + 2) * keys * sizeof(int), s, ids, entries, chunk, groups, key_bits,
-                     blocks > 1 ? table : nullptr, blocks, per_row, order, offsets, place, rows);
+  hipLaunchKernelGGL(group_count_kernel<Id>, dim3(blocks), dim3(kGroupThreads), kGroupWaves * keys * sizeof(int), s, ids, entries, chunk, groups, key_bits, table);
+  EP_HIP_TRY(hipGetLastError());
+  if (chunk == kGroupChunk)
+    hipLaunchKernelGGL((group_place_kernel<Id, 4>), dim3(blocks), dim3(kGroupThreads), room, s, ids, entries, chunk, groups, key_bits, table, blocks, out);
+  else
+    hipLaunchKernelGGL((group_place_kernel<Id, 0>), dim3(blocks), dim3(kGroupThreads), room, s, ids, entries, chunk, groups, key_bits, table, blocks, out);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
 }
@@ -311,7 +365,7 @@ extern "C" {
 size_t ep_hip_group_rows_workspace(int64_t entries, int groups) {
   if (entries <= 0 || groups <= 0) return 0;
   const int64_t chunk = ep::group_chunk(entries), blocks = (entries + chunk - 1) / chunk;
-  return blocks > 1 ? static_cast<size_t>(blocks) * static_cast<size_t>(groups + 1) * 4 : 0;
+  return entries > ep::kOneBlock ? static_cast<size_t>(blocks) * static_cast<size_t>(groups + 1) * 4 : 0;
 }
 
 int ep_hip_group_rows(const void* ids_dev, int id_bytes, int64_t entries, int groups, int per_row, int32_t* order_dev, int32_t* offsets_dev, int32_t* place_dev,
@@ -324,8 +378,9 @@ int ep_hip_group_rows(const void* ids_dev, int id_bytes, int64_t entries, int gr
   if (wanted != 0 && (workspace_dev == nullptr || workspace_bytes < wanted)) return EP_HIP_EINVAL;
   int32_t* table = static_cast<int32_t*>(workspace_dev);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (id_bytes == 4) return launch_group(static_cast<const int32_t*>(ids_dev), entries, groups, per_row, order_dev, offsets_dev, place_dev, rows_dev, table, s);
-  return launch_group(static_cast<const int64_t*>(ids_dev), entries, groups, per_row, order_dev, offsets_dev, place_dev, rows_dev, table, s);
+  const GroupOut out = {order_dev, offsets_dev, place_dev, rows_dev, per_row};
+  if (id_bytes == 4) return launch_group(static_cast<const int32_t*>(ids_dev), entries, groups, out, table, s);
+  return launch_group(static_cast<const int64_t*>(ids_dev), entries, groups, out, table, s);
 }
 
 int ep_hip_combine_rows(const void* y_dev, int y_kind, int64_t ldy, const int32_t* place_dev, const int32_t* kept_rows_dev, const void* weight_dev, int weight_kind,

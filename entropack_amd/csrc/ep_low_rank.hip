@@ -204,43 +204,76 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
 // transposed. The products are the weights' gradient of ep_grouped_tile.hpp with the planes as left operand. They are bound by
 // reading q, and the groups alone make too few tiles to fill the card, so the places of every group are divided into chunks, each
 // chunk writes its f32 sums to a matrix of its own, and this kernel adds a group's chunks in their order and rounds once.
-// A block takes 64 columns of one group, 64 ranks at a time.
-__global__ __launch_bounds__(256) void low_rank_finish_kernel(const float* __restrict__ parts, int chunk, int padded, int rank, const int32_t* __restrict__ offsets,
-                                                              int width, uint16_t* __restrict__ out, int transposed) {
-  __shared__ uint16_t turned[64][66];
-  const int column_tiles = (width + 63) / 64;
-  const int group = static_cast<int>(blockIdx.x / column_tiles), n0 = static_cast<int>(blockIdx.x % column_tiles) * 64;
+// A block takes 64 columns and 16 ranks of one group, a wave one of the ranks.
+__global__ __launch_bounds__(1024) void low_rank_finish_kernel(const float* __restrict__ parts, int chunk, int padded, int rank, const int32_t* __restrict__ offsets,
+                                                               int width, uint16_t* __restrict__ out, int transposed) {
+  __shared__ uint16_t turned[64][18];
+  const int column_tiles = (width + 63) / 64, rank_tiles = padded / 16;
+  const int at = static_cast<int>(blockIdx.x / column_tiles), n0 = static_cast<int>(blockIdx.x % column_tiles) * 64;
+  const int group = at / rank_tiles, e0 = at % rank_tiles * 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // The chunks of the groups before this one, and this one's.
   int before = 0;
   for (int g = lane; g < group; g += 64) before += (offsets[g + 1] - offsets[g] + chunk - 1) / chunk;
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d);
+  before = __builtin_amdgcn_readlane(wave_inclusive_sum(before), 63);
   const int chunks = (offsets[group + 1] - offsets[group] + chunk - 1) / chunk;
   const int64_t matrix = static_cast<int64_t>(2 * padded) * width;
-  const float* from = parts + before * matrix;
-  const int n = n0 + lane;
-  for (int e0 = 0; e0 < rank; e0 += 64) {
-    const int ranks = rank - e0 < 64 ? rank - e0 : 64;
-    for (int e = wave; e < ranks; e += 4) {
-      float sum = 0.0f;
-      if (n < width) {
-        const float* high = from + static_cast<int64_t>(e0 + e) * width + n;
-        const float* low = high + static_cast<int64_t>(padded) * width;
+  const int n = n0 + lane, e = e0 + wave;
+  float sum = 0.0f;
+  if (n < width) {
+    const float* high = parts + before * matrix + static_cast<int64_t>(e) * width + n;
+    const float* low = high + static_cast<int64_t>(padded) * width;
 #pragma unroll 4
-        for (int c = 0; c < chunks; ++c) sum += high[c * matrix] + low[c * matrix];
-      }
-      const uint16_t bits = static_cast<uint16_t>(bf16_bits_of(sum));
-      if (transposed) turned[lane][e] = bits;
-      else if (n < width) out[(static_cast<int64_t>(group) * rank + e0 + e) * width + n] = bits;
-    }
-    if (transposed) {
-      __syncthreads();
-      const int columns = width - n0 < 64 ? width - n0 : 64;
-      for (int cell = threadIdx.x; cell < columns * ranks; cell += 256)
-        out[(static_cast<int64_t>(group) * width + n0 + cell / ranks) * rank + e0 + cell % ranks] = turned[cell / ranks][cell % ranks];
-      __syncthreads();
-    }
+    for (int c = 0; c < chunks; ++c) sum += high[c * matrix] + low[c * matrix];
+  }
+  const uint16_t bits = static_cast<uint16_t>(bf16_bits_of(sum));
+  if (!transposed) {
+    if (n < width && e < rank) out[(static_cast<int64_t>(group) * rank + e) * width + n] = bits;
+    return;
+  }
+  turned[lane][wave] = bits;
+  __syncthreads();
+  const int column = n0 + (threadIdx.x >> 4), of = e0 + (threadIdx.x & 15);
+  if (column < width && of < rank) out[(static_cast<int64_t>(group) * width + column) * rank + of] = turned[threadIdx.x >> 4][threadIdx.x & 15];
+}
+
+// Both transposes that the gradients need, [groups][rows][columns] to [groups][columns][out_rows] with zeros in rows .. out_rows: 64 x 64
+// blocks by way of LDS, those of the first matrix before those of the second.
+struct Transpose {
+  const uint16_t* in;
+  uint16_t* out;
+  int64_t ld, group;
+  int rows, columns, out_rows;
+  int row_tiles, column_tiles;     // of 64; rows counted to out_rows
+};
+
+__global__ __launch_bounds__(256) void low_rank_transpose_kernel(Transpose first, Transpose second, int first_blocks) {
+  __shared__ uint16_t turned[64][66];
+  const bool of_first = static_cast<int>(blockIdx.x) < first_blocks;
+  const Transpose t = of_first ? first : second;
+  const int block = static_cast<int>(blockIdx.x) - (of_first ? 0 : first_blocks);
+  const int column0 = block % t.column_tiles * 64, row0 = block / t.column_tiles % t.row_tiles * 64;
+  const int64_t group = block / t.column_tiles / t.row_tiles;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int column = column0 + lane;
+  const uint16_t* in = t.in + group * t.group + (column < t.columns ? column : 0);
+  uint16_t held[16];                             // all loads before the first is used; those outside read row or column 0
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = row0 + 4 * i + wave;
+    held[i] = in[(row < t.rows ? row : 0) * t.ld];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = row0 + 4 * i + wave;
+    turned[lane][4 * i + wave] = row < t.rows && column < t.columns ? held[i] : 0;
+  }
+  __syncthreads();
+  uint16_t* out = t.out + group * t.columns * t.out_rows;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int turned_row = column0 + 4 * i + wave, at = row0 + lane;
+    if (turned_row < t.columns && at < t.out_rows) out[static_cast<int64_t>(turned_row) * t.out_rows + at] = turned[4 * i + wave][lane];
   }
 }
 
@@ -257,58 +290,50 @@ static int64_t reduce_chunks(int64_t entries, int groups, int chunk) {       // 
   return entries / chunk + (groups < entries ? groups : entries);
 }
 
-static bool low_rank_valid(const int32_t* order, const int32_t* offsets, int64_t entries, int groups, int64_t rows, int64_t rank, int64_t width) {
-  return order != nullptr && offsets != nullptr && entries > 0 && entries <= kMostEntries && groups > 0 && rows == entries && rank > 0 && rank <= 4096 && width > 0 &&
-         width <= 0x3FFFFFFF / groups;
-}
+static int padded_rank(int64_t rank) { return static_cast<int>((rank + 15) / 16 * 16); }
+static int64_t whole_pieces(int64_t elements) { return (elements + 7) / 8 * 8; }
+static size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
+static size_t planes_bytes(int64_t entries, int64_t rank) { return static_cast<size_t>(entries) * static_cast<size_t>(padded_rank(rank)) * 4; }
 
-}  // namespace ep
+// The adapters and the rows they are for.
+struct Grouping {
+  const int32_t* order;
+  const int32_t* offsets;
+  int64_t entries;
+  int groups;
+};
 
-extern "C" {
-
-size_t ep_hip_low_rank_planes_bytes(int64_t entries, int64_t rank) {
-  if (entries <= 0 || rank <= 0) return 0;
-  return static_cast<size_t>(entries) * static_cast<size_t>((rank + 15) / 16 * 16) * 4;
-}
-
-int ep_hip_low_rank_shrink(const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group, const float* scale_dev, void* planes_dev,
-                           const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t K, void* stream) {
-  using namespace ep;
-  if (x_dev == nullptr || down_dev == nullptr || planes_dev == nullptr || !low_rank_valid(order_dev, offsets_dev, entries, groups, entries, rank, K)) return EP_HIP_EINVAL;
-  if (K % 8 != 0 || ldx % 8 != 0 || ldd % 8 != 0 || down_group % 8 != 0 || ldx < K || ldd < K || down_group < 0) return EP_HIP_EINVAL;
-  if (reinterpret_cast<uintptr_t>(x_dev) % 16 != 0 || reinterpret_cast<uintptr_t>(down_dev) % 16 != 0 || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
+// planes[p] = scale[a] x[order[p]] . down[a]^T; K a whole number of pieces.
+static int shrink(const Grouping& g, const void* x, int64_t ldx, const void* down, int64_t ldd, int64_t down_group, const float* scale, void* planes, int64_t rank, int64_t K,
+                  hipStream_t s) {
   GroupedArgs a = {};
-  a.x = static_cast<const uint8_t*>(x_dev), a.w = static_cast<const uint8_t*>(down_dev), a.scale_x = scale_dev, a.y = planes_dev, a.row_of = order_dev, a.offsets = offsets_dev;
-  a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = (rank + 15) / 16 * 16 * 2;
-  a.entries = static_cast<int>(entries), a.groups = groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(entries), a.out_kind = kOutBF16;
+  a.x = static_cast<const uint8_t*>(x), a.w = static_cast<const uint8_t*>(down), a.scale_x = scale, a.y = planes, a.row_of = g.order, a.offsets = g.offsets;
+  a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = 2 * padded_rank(rank);
+  a.entries = static_cast<int>(g.entries), a.groups = g.groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(g.entries), a.out_kind = kOutBF16;
   // All of a rank up to 64 in one block, so that x is read once. 4099 rows of 4096: rank 16 9.0 us (8 waves 10.5; 500 rows 6.0 against
   // 5.4), rank 64 16.1 us (32 ranks per block 19.2); 7993 rows, rank 32, 18.5 us (16 rows per block 19.6; reading x takes 10.6).
-  hipStream_t s = static_cast<hipStream_t>(stream);
   if (rank > 32) return launch_stream_of<false, 2, 4, 4, true>(a, s);
   if (rank > 16) return launch_stream_of<false, 2, 2, 8, true>(a, s);
-  return entries >= 2048 ? launch_stream_of<false, 1, 1, 4, true>(a, s) : launch_stream_of<false, 1, 1, 8, true>(a, s);
+  return g.entries >= 2048 ? launch_stream_of<false, 1, 1, 4, true>(a, s) : launch_stream_of<false, 1, 1, 8, true>(a, s);
 }
 
-int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t ldu, int64_t up_group, const void* y_dev, int64_t ldy, void* out_dev, int64_t ldo,
-                           const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t N, void* stream) {
-  using namespace ep;
-  if (planes_dev == nullptr || up_dev == nullptr || out_dev == nullptr || !low_rank_valid(order_dev, offsets_dev, entries, groups, entries, rank, N)) return EP_HIP_EINVAL;
-  if (ldu < rank || up_group < 0 || ldo < N || (y_dev != nullptr && ldy < N) || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
+// out[order[p]] = y[order[p]] + planes[p] . up[a]^T, rows of no group as in y.
+static int expand(const Grouping& g, const void* planes, const void* up, int64_t ldu, int64_t up_group, const void* y, int64_t ldy, void* out, int64_t ldo, int64_t rank,
+                  int64_t N, hipStream_t s) {
   LowRankArgs a = {};
-  a.planes = static_cast<const uint16_t*>(planes_dev), a.up = static_cast<const uint16_t*>(up_dev), a.y = static_cast<const uint16_t*>(y_dev);
-  a.out = static_cast<uint16_t*>(out_dev), a.order = order_dev, a.offsets = offsets_dev;
+  a.planes = static_cast<const uint16_t*>(planes), a.up = static_cast<const uint16_t*>(up), a.y = static_cast<const uint16_t*>(y);
+  a.out = static_cast<uint16_t*>(out), a.order = g.order, a.offsets = g.offsets;
   a.ldu = ldu, a.up_group = up_group, a.ldy = ldy, a.ldo = ldo;
-  a.entries = static_cast<int>(entries), a.groups = groups, a.rank = static_cast<int>(rank), a.padded = static_cast<int>((rank + 15) / 16 * 16), a.N = static_cast<int>(N);
-  a.rows = static_cast<int>(entries);
+  a.entries = static_cast<int>(g.entries), a.groups = g.groups, a.rank = static_cast<int>(rank), a.padded = padded_rank(rank), a.N = static_cast<int>(N);
+  a.rows = static_cast<int>(g.entries);
   auto in_pieces = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
-  const bool pieces = in_pieces(up_dev, ldu) && up_group % 8 == 0 && rank % 8 == 0;
-  const bool wide = in_pieces(out_dev, ldo) && N % 8 == 0 && (y_dev == nullptr || in_pieces(y_dev, ldy));
-  const bool tall = entries / groups >= 32;                  // most blocks of 64 rows are then at least half full
+  const bool pieces = in_pieces(up, ldu) && up_group % 8 == 0 && rank % 8 == 0;
+  const bool wide = in_pieces(out, ldo) && N % 8 == 0 && (y == nullptr || in_pieces(y, ldy));
+  const bool tall = g.entries / g.groups >= 32;              // most blocks of 64 rows are then at least half full
   const int columns = tall ? kTallColumns : 256;
-  const int64_t blocks = most_row_tiles(entries, groups, tall ? 64 : 16) * ((N + columns - 1) / columns);
+  const int64_t blocks = most_row_tiles(g.entries, g.groups, tall ? 64 : 16) * ((N + columns - 1) / columns);
   if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
-  hipStream_t s = static_cast<hipStream_t>(stream);
 #define EP_EXPAND(PIECES, WIDE)                                                                                               \
   if (!tall) hipLaunchKernelGGL((low_rank_expand_kernel<PIECES, WIDE>), grid, dim3(256), 0, s, a);                             \
   else if (a.padded <= 16) hipLaunchKernelGGL((low_rank_expand_tall_kernel<PIECES, WIDE, 16>), grid, dim3(256), 0, s, a);      \
@@ -328,35 +353,119 @@ int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t l
   return EP_HIP_OK;
 }
 
-size_t ep_hip_low_rank_reduce_workspace(int64_t entries, int groups, int64_t rank, int64_t width) {
-  using namespace ep;
-  if (entries <= 0 || groups <= 0 || rank <= 0 || width <= 0) return 0;
-  return static_cast<size_t>(reduce_chunks(entries, groups, reduce_chunk(entries, rank, width))) * static_cast<size_t>((rank + 15) / 16 * 32) * static_cast<size_t>(width) * 4;
+static size_t reduce_bytes(int64_t entries, int groups, int64_t rank, int64_t width) {
+  return static_cast<size_t>(reduce_chunks(entries, groups, reduce_chunk(entries, rank, width))) * static_cast<size_t>(2 * padded_rank(rank)) * static_cast<size_t>(width) * 4;
 }
 
-int ep_hip_low_rank_reduce(const void* planes_dev, const void* q_dev, int64_t ldq, void* out_dev, int transposed, const int32_t* order_dev, const int32_t* offsets_dev,
-                           int64_t entries, int groups, int64_t rank, int64_t width, void* workspace_dev, size_t workspace_bytes, void* stream) {
-  using namespace ep;
-  if (planes_dev == nullptr || q_dev == nullptr || out_dev == nullptr || workspace_dev == nullptr) return EP_HIP_EINVAL;
-  if (!low_rank_valid(order_dev, offsets_dev, entries, groups, entries, rank, width)) return EP_HIP_EINVAL;
-  const int64_t readable = (width + 7) / 8 * 8;
-  if (ldq < readable || ldq % 8 != 0 || reinterpret_cast<uintptr_t>(q_dev) % 16 != 0 || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
-  if (reinterpret_cast<uintptr_t>(workspace_dev) % 16 != 0 || workspace_bytes < ep_hip_low_rank_reduce_workspace(entries, groups, rank, width)) return EP_HIP_EINVAL;
-  const int padded = static_cast<int>((rank + 15) / 16 * 16);
+// out[a][e][n] (transposed: out[a][n][e]) = sum over a's places of planes[p][e] q[order[p]][n]; rows of q readable to a whole number of pieces.
+static int reduce(const Grouping& g, const void* planes, const void* q, int64_t ldq, void* out, bool transposed, int64_t rank, int64_t width, void* parts, hipStream_t s) {
+  const int padded = padded_rank(rank);
   TileArgs t = {};
-  t.a = static_cast<const uint8_t*>(planes_dev), t.b = static_cast<const uint8_t*>(q_dev), t.y = workspace_dev, t.row_of = order_dev, t.offsets = offsets_dev;
+  t.a = static_cast<const uint8_t*>(planes), t.b = static_cast<const uint8_t*>(q), t.y = parts, t.row_of = g.order, t.offsets = g.offsets;
   t.lda_bytes = padded * int64_t{4}, t.ldb_bytes = ldq * 2, t.ldy = width, t.group_y = 2 * padded * width;
-  t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(entries), t.out_kind = kOutF32;
-  t.rows = 2 * padded, t.columns = static_cast<int>(width), t.chunk = reduce_chunk(entries, rank, width);
-  const int64_t blocks = reduce_chunks(entries, groups, t.chunk) * ((t.rows + kTile - 1) / kTile) * ((width + kTile - 1) / kTile);
-  const int64_t finish = groups * ((width + 63) / 64);
+  t.entries = static_cast<int>(g.entries), t.groups = g.groups, t.x_rows = static_cast<int>(g.entries), t.out_kind = kOutF32;
+  t.rows = 2 * padded, t.columns = static_cast<int>(width), t.chunk = reduce_chunk(g.entries, rank, width);
+  const int64_t blocks = reduce_chunks(g.entries, g.groups, t.chunk) * ((t.rows + kTile - 1) / kTile) * ((width + kTile - 1) / kTile);
+  const int64_t finish = static_cast<int64_t>(g.groups) * (padded / 16) * ((width + 63) / 64);
   if (blocks > 0x7FFFFFFF || finish > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
-  hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL((grouped_tile_kernel<false, kGradWeight, true, true>), dim3(static_cast<unsigned>(blocks)), dim3(kTileThreads), 0, s, t);
   EP_HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(low_rank_finish_kernel, dim3(static_cast<unsigned>(finish)), dim3(256), 0, s, static_cast<const float*>(workspace_dev), t.chunk, padded,
-                     static_cast<int>(rank), offsets_dev, static_cast<int>(width), static_cast<uint16_t*>(out_dev), transposed);
+  hipLaunchKernelGGL(low_rank_finish_kernel, dim3(static_cast<unsigned>(finish)), dim3(1024), 0, s, static_cast<const float*>(parts), t.chunk, padded, static_cast<int>(rank),
+                     g.offsets, static_cast<int>(width), static_cast<uint16_t*>(out), transposed ? 1 : 0);
   EP_HIP_TRY(hipGetLastError());
+  return EP_HIP_OK;
+}
+
+// Where the gradients keep what lies between their products: both transposes, the planes of the output's gradient, the chunks' sums.
+struct GradRoom {
+  size_t up_turned, down_turned, planes, parts, bytes;
+};
+
+static GradRoom grad_room(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N) {
+  GradRoom r;
+  const size_t g = static_cast<size_t>(groups);
+  r.up_turned = 0;                                                                         // [groups][rank][whole pieces of N]
+  r.down_turned = r.up_turned + whole_lines(g * static_cast<size_t>(rank * whole_pieces(N)) * 2);     // [groups][K][whole pieces of rank]
+  r.planes = r.down_turned + whole_lines(g * static_cast<size_t>(K * whole_pieces(rank)) * 2);
+  r.parts = r.planes + whole_lines(planes_bytes(entries, rank));
+  const size_t of_down = reduce_bytes(entries, groups, rank, K), of_up = reduce_bytes(entries, groups, rank, N);
+  r.bytes = r.parts + (of_down > of_up ? of_down : of_up);
+  return r;
+}
+
+static bool low_rank_valid(const Grouping& g, int64_t rank, int64_t K, int64_t N) {
+  return g.order != nullptr && g.offsets != nullptr && g.entries > 0 && g.entries <= kMostEntries && g.groups > 0 && rank > 0 && rank <= 4096 && K > 0 && N > 0 &&
+         K <= 0x3FFFFF00 / g.groups && N <= 0x3FFFFF00 / g.groups;
+}
+
+// Rows read in whole 16-byte pieces, the last one zero from `width` on.
+static bool rows_in_pieces(const void* base, int64_t ld, int64_t width) {
+  return base != nullptr && reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld % 8 == 0 && ld >= whole_pieces(width);
+}
+
+}  // namespace ep
+
+extern "C" {
+
+size_t ep_hip_low_rank_planes_bytes(int64_t entries, int64_t rank) { return entries <= 0 || rank <= 0 ? 0 : ep::planes_bytes(entries, rank); }
+
+int ep_hip_low_rank_update(const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group, const void* up_dev, int64_t ldu, int64_t up_group,
+                           const float* scale_dev, const void* y_dev, int64_t ldy, void* planes_dev, void* out_dev, int64_t ldo, const int32_t* order_dev,
+                           const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t K, int64_t N, void* stream) {
+  using namespace ep;
+  const Grouping g = {order_dev, offsets_dev, entries, groups};
+  if (!low_rank_valid(g, rank, K, N) || planes_dev == nullptr || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
+  if (!rows_in_pieces(x_dev, ldx, K) || !rows_in_pieces(down_dev, ldd, K) || down_group % 8 != 0 || down_group < 0) return EP_HIP_EINVAL;
+  if (up_dev == nullptr || out_dev == nullptr || ldu < rank || up_group < 0 || ldo < N || (y_dev != nullptr && ldy < N)) return EP_HIP_EINVAL;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int status = shrink(g, x_dev, ldx, down_dev, ldd, down_group, scale_dev, planes_dev, rank, whole_pieces(K), s);
+  return status != EP_HIP_OK ? status : expand(g, planes_dev, up_dev, ldu, up_group, y_dev, ldy, out_dev, ldo, rank, N, s);
+}
+
+size_t ep_hip_low_rank_grad_workspace(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N) {
+  if (entries <= 0 || groups <= 0 || rank <= 0 || K <= 0 || N <= 0) return 0;
+  return ep::grad_room(entries, groups, rank, K, N).bytes;
+}
+
+int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group,
+                                const void* up_dev, int64_t ldu, int64_t up_group, const float* scale_dev, const void* planes_dev, void* grad_x_dev, int64_t ldgx,
+                                void* grad_down_dev, void* grad_up_dev, const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank,
+                                int64_t K, int64_t N, void* workspace_dev, size_t workspace_bytes, void* stream) {
+  using namespace ep;
+  const Grouping g = {order_dev, offsets_dev, entries, groups};
+  if (!low_rank_valid(g, rank, K, N) || !rows_in_pieces(grad_dev, ldg, N)) return EP_HIP_EINVAL;
+  if (grad_x_dev == nullptr && grad_down_dev == nullptr && grad_up_dev == nullptr) return EP_HIP_EINVAL;
+  const bool back = grad_x_dev != nullptr || grad_down_dev != nullptr;         // the narrow rows' gradient is needed
+  if (back && (up_dev == nullptr || ldu < rank || up_group < 0)) return EP_HIP_EINVAL;
+  if (grad_x_dev != nullptr && (down_dev == nullptr || ldd < K || down_group < 0 || ldgx < K)) return EP_HIP_EINVAL;
+  if (grad_down_dev != nullptr && !rows_in_pieces(x_dev, ldx, K)) return EP_HIP_EINVAL;
+  if (grad_up_dev != nullptr && (planes_dev == nullptr || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0)) return EP_HIP_EINVAL;
+  const GradRoom room = grad_room(entries, groups, rank, K, N);
+  if (workspace_dev == nullptr || reinterpret_cast<uintptr_t>(workspace_dev) % 256 != 0 || workspace_bytes < room.bytes) return EP_HIP_EINVAL;
+  uint8_t* const base = static_cast<uint8_t*>(workspace_dev);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (back) {
+    // The gradient of the narrow rows is a shrink by up^T, that of x an expand by down^T.
+    auto tiles = [](Transpose& t) { return t.column_tiles = (t.columns + 63) / 64, t.row_tiles = (t.out_rows + 63) / 64, static_cast<int64_t>(t.column_tiles) * t.row_tiles; };
+    Transpose up = {static_cast<const uint16_t*>(up_dev), reinterpret_cast<uint16_t*>(base + room.up_turned), ldu, up_group, static_cast<int>(N), static_cast<int>(rank),
+                    static_cast<int>(whole_pieces(N)), 0, 0};
+    Transpose down = {static_cast<const uint16_t*>(down_dev), reinterpret_cast<uint16_t*>(base + room.down_turned), ldd, down_group, static_cast<int>(rank), static_cast<int>(K),
+                      static_cast<int>(whole_pieces(rank)), 0, 0};
+    const int64_t first = tiles(up) * groups, second = tiles(down) * (grad_x_dev != nullptr ? groups : 0);
+    if (first + second > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+    hipLaunchKernelGGL(low_rank_transpose_kernel, dim3(static_cast<unsigned>(first + second)), dim3(256), 0, s, up, down, static_cast<int>(first));
+    EP_HIP_TRY(hipGetLastError());
+    const int64_t turned = whole_pieces(N);
+    if (const int status = shrink(g, grad_dev, ldg, base + room.up_turned, turned, rank * turned, scale_dev, base + room.planes, rank, turned, s)) return status;
+    if (grad_x_dev != nullptr) {
+      const int64_t ranks = whole_pieces(rank);
+      if (const int status = expand(g, base + room.planes, base + room.down_turned, ranks, K * ranks, nullptr, 0, grad_x_dev, ldgx, rank, K, s)) return status;
+    }
+    if (grad_down_dev != nullptr) {
+      if (const int status = reduce(g, base + room.planes, x_dev, ldx, grad_down_dev, false, rank, K, base + room.parts, s)) return status;
+    }
+  }
+  if (grad_up_dev != nullptr) return reduce(g, planes_dev, grad_dev, ldg, grad_up_dev, true, rank, N, base + room.parts, s);
   return EP_HIP_OK;
 }
 

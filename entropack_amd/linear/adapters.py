@@ -10,53 +10,27 @@ from __future__ import annotations
 import torch
 
 from ..backends import hip as _hip
-from .groups import RowGroups, device_of, matrix
+from .groups import RowGroups, device_of, matrix, rows_of
 from .linear import CompressedLinear
 
 
-def _shrink(x, down, scale, groups: RowGroups) -> torch.Tensor:
-    """scale[a] * x down[a]^T per place, as two bf16 parts (value, remainder) of `rank` rounded up to 16 columns each."""
-    rank = down.shape[1]
+def _update(y, x, down, up, scale, groups: RowGroups) -> tuple[torch.Tensor, torch.Tensor]:
+    """The updated rows, and the narrow rows between the two products (two bf16 parts of the rank rounded up to 16 each)."""
+    rank, outer = up.shape[2], up.shape[1]
     planes = torch.empty(groups.entries, 2 * (-(-rank // 16) * 16), dtype=torch.bfloat16, device=x.device)
-    rows, narrow = matrix(x, 8), matrix(down, 8)
-    _hip.launch("ep_hip_low_rank_shrink", x.device,
-                rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0), None if scale is None else scale.data_ptr(),
-                planes.data_ptr(), groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, rows.shape[1])
-    return planes
-
-
-def _expand(planes, up, y, groups: RowGroups) -> torch.Tensor:
-    """y + planes up[a]^T, rows of no group as they are in y (zero where y is None)."""
-    outer, rank = up.shape[1], up.shape[2]
-    if not (up.stride(2) == 1 and up.stride(1) >= rank and up.stride(0) >= outer * up.stride(1)):
-        up = up.contiguous()
-    out = torch.empty(groups.entries, outer, dtype=torch.bfloat16, device=planes.device)
-    if y is not None and not (y.stride(1) == 1 and y.stride(0) >= outer):
-        y = y.contiguous()
-    _hip.launch("ep_hip_low_rank_expand", planes.device,
-                planes.data_ptr(), up.data_ptr(), up.stride(1), up.stride(0), None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
-                out.data_ptr(), outer, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, outer)
-    return out
-
-
-def _reduce(planes, rank: int, rows, transposed: bool, groups: RowGroups) -> torch.Tensor:
-    """Per adapter the sum over its places of planes^T rows: [adapters, rank, width], or [adapters, width, rank] transposed."""
-    width = rows.shape[1]
-    rows = matrix(rows, 8)
-    out = torch.empty((groups.groups, width, rank) if transposed else (groups.groups, rank, width), dtype=torch.bfloat16, device=planes.device)
-    room = _hip.library().ep_hip_low_rank_reduce_workspace(groups.entries, groups.groups, rank, width)
-    workspace = torch.empty(room, dtype=torch.uint8, device=planes.device)
-    _hip.launch("ep_hip_low_rank_reduce", planes.device,
-                planes.data_ptr(), rows.data_ptr(), rows.stride(0), out.data_ptr(), int(transposed), groups.order.data_ptr(), groups.offsets.data_ptr(),
-                groups.entries, groups.groups, rank, width, workspace.data_ptr(), room)
-    return out
+    out = torch.empty(groups.entries, outer, dtype=torch.bfloat16, device=x.device)
+    rows, narrow, wide, base = matrix(x, 8), matrix(down, 8), rows_of(up), rows_of(y)
+    _hip.launch("ep_hip_low_rank_update", x.device,
+                rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0), wide.data_ptr(), wide.stride(1), wide.stride(0),
+                None if scale is None else scale.data_ptr(), base.data_ptr(), base.stride(0), planes.data_ptr(), out.data_ptr(), outer,
+                groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, x.shape[1], outer)
+    return out, planes
 
 
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, down, up, scale, groups):
-        planes = _shrink(x, down, scale, groups)
-        out = _expand(planes, up, y, groups)
+        out, planes = _update(y, x, down, up, scale, groups)
         ctx.groups = groups
         ctx.save_for_backward(x, down, up, scale, planes if ctx.needs_input_grad[3] else None)
         return out
@@ -66,16 +40,21 @@ class _LowRankUpdate(torch.autograd.Function):
     def backward(ctx, grad):
         x, down, up, scale, planes = ctx.saved_tensors
         groups, (need_y, need_x, need_down, need_up) = ctx.groups, ctx.needs_input_grad[:4]
-        grad_x = grad_down = grad_up = None
-        if need_x or need_down:
-            # The gradient of the narrow rows is a shrink by up^T, that of x an expand by down^T: two small transposes.
-            narrow = _shrink(grad, up.transpose(1, 2).contiguous(), scale, groups)
-            if need_x:
-                grad_x = _expand(narrow, down.transpose(1, 2).contiguous(), None, groups)
-            if need_down:
-                grad_down = _reduce(narrow, down.shape[1], x, False, groups)
-        if need_up:
-            grad_up = _reduce(planes, up.shape[2], grad, True, groups)
+        grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        grad_down = torch.empty(down.shape, dtype=down.dtype, device=x.device) if need_down else None
+        grad_up = torch.empty(up.shape, dtype=up.dtype, device=x.device) if need_up else None
+        if need_x or need_down or need_up:
+            inner, outer, rank = x.shape[1], up.shape[1], up.shape[2]
+            room = _hip.library().ep_hip_low_rank_grad_workspace(groups.entries, groups.groups, rank, inner, outer)
+            workspace = torch.empty(room, dtype=torch.uint8, device=x.device)
+            slope, rows, narrow, wide = matrix(grad, 8), matrix(x, 8), rows_of(down), rows_of(up)
+            _hip.launch("ep_hip_low_rank_update_grad", x.device,
+                        slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0),
+                        wide.data_ptr(), wide.stride(1), wide.stride(0), None if scale is None else scale.data_ptr(),
+                        None if planes is None else planes.data_ptr(), None if grad_x is None else grad_x.data_ptr(), inner,
+                        None if grad_down is None else grad_down.data_ptr(), None if grad_up is None else grad_up.data_ptr(),
+                        groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, inner, outer,
+                        workspace.data_ptr(), room)
         return grad if need_y else None, grad_x, grad_down, grad_up, None, None
 
 
@@ -121,7 +100,7 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         return y + (x.sum() + down.sum() + up.sum()) * 0
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or down.requires_grad or up.requires_grad):
         return _LowRankUpdate.apply(y, x, down, up, scale, groups)
-    return _expand(_shrink(x, down, scale, groups), up, y, groups)
+    return _update(y, x, down, up, scale, groups)[0]
 
 
 class AdaptedLinear(torch.nn.Module):

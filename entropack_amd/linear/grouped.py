@@ -17,7 +17,7 @@ import torch
 from ..backends import hip as _hip
 from ..compression import BatchDecompressor
 from . import kernels
-from .groups import RowGroups, device_of, matrix, sum_entries
+from .groups import RowGroups, device_of, matrix, rows_of, sum_entries
 from .linear import CompressedINT8Linear, CompressedLinear
 
 
@@ -85,7 +85,7 @@ def _grad_bias(grad, groups: RowGroups) -> torch.Tensor:
     outer = grad.shape[1]
     if groups.entries == 0:
         return torch.zeros(groups.groups, outer, dtype=torch.bfloat16, device=grad.device)
-    dy = grad if grad.stride(1) == 1 and grad.stride(0) >= outer else grad.contiguous()
+    dy = rows_of(grad)
     out = torch.empty(groups.groups, outer, dtype=torch.bfloat16, device=grad.device)
     _hip.launch("ep_hip_grouped_column_sums_bf16", grad.device,
                 dy.data_ptr(), dy.stride(0), groups.offsets.data_ptr(), groups.groups, outer, out.data_ptr(),
@@ -238,9 +238,11 @@ class CompressedGroupedLinear(torch.nn.Module):
             held = self._decoder = (payloads, BatchDecompressor(containers, self.experts[0]._decode_config))
         arena = torch.empty(held[1].arena_bytes, dtype=torch.uint8, device=device)
         views = held[1](arena)
-        apart = 0 if len(views) == 1 else (views[1].data_ptr() - views[0].data_ptr()) // views[0].element_size()
-        row = views[0].stride(0)
-        return torch.as_strided(views[0], (len(views), self.out_features, self.in_features), (apart or row * self.out_features, row, 1))
+        if any(view.untyped_storage().data_ptr() != arena.data_ptr() for view in views):
+            return torch.stack(views)                        # a type the decode stores as another and converts
+        size, row = views[0].element_size(), views[0].stride(0)
+        apart = row * self.out_features if len(views) == 1 else (views[1].data_ptr() - views[0].data_ptr()) // size    # one shape, so even steps
+        return torch.as_strided(views[0], (len(views), self.out_features, self.in_features), (apart, row, 1))
 
     def _product(self, x: torch.Tensor, groups: RowGroups, x_grouped: bool) -> torch.Tensor:
         weight = self._stacked(x.device)

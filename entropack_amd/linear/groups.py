@@ -52,6 +52,16 @@ def matrix(tensor: torch.Tensor, pieces: int) -> torch.Tensor:
     return tensor if fits else tensor.clone(memory_format=torch.contiguous_format)
 
 
+def rows_of(tensor: torch.Tensor) -> torch.Tensor:
+    """`tensor` ([.., columns]) for kernels that take any address: columns contiguous, rows and groups not overlapping."""
+    fits = tensor.stride(-1) == 1
+    least = tensor.shape[-1]
+    for dim in range(tensor.dim() - 2, -1, -1):
+        fits = fits and tensor.stride(dim) >= least
+        least = tensor.stride(dim) * (tensor.shape[dim] - 1) + least
+    return tensor if fits else tensor.clone(memory_format=torch.contiguous_format)
+
+
 @dataclasses.dataclass(frozen=True, eq=False)
 class RowGroups:
     """What `group_rows` made of a tensor of ids. Made by `group_rows` only: the kernels take its indices as they are.
@@ -130,13 +140,8 @@ def sum_entries(rows: torch.Tensor, tokens: int, per_row: int) -> torch.Tensor:
     return out
 
 
-def _rows_of(tensor: torch.Tensor) -> torch.Tensor:
-    """Rows at any address the element-wise kernels take: columns contiguous, rows not overlapping."""
-    return tensor if tensor.stride(1) == 1 and tensor.stride(0) >= tensor.shape[1] else tensor.contiguous()
-
-
 def _combine(y, weight, groups: RowGroups) -> torch.Tensor:
-    rows = _rows_of(y)
+    rows = rows_of(y)
     ready = None if weight is None else weight.contiguous()
     out = torch.empty(groups.tokens, y.shape[1], dtype=torch.bfloat16, device=y.device)
     if out.numel():
@@ -162,7 +167,7 @@ class _CombineRows(torch.autograd.Function):
         grad_y = torch.empty_like(y, memory_format=torch.contiguous_format) if need_y else None
         grad_weight = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_weight else None
         if y.numel():
-            rows, ready, slope = _rows_of(y), None if weight is None else weight.contiguous(), _rows_of(grad)
+            rows, ready, slope = rows_of(y), None if weight is None else weight.contiguous(), rows_of(grad)
             _hip.launch("ep_hip_combine_rows_grad", y.device,
                         slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
                         None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,

@@ -462,21 +462,24 @@ int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void
                                     int64_t K, void* stream);
 int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int32_t* offsets_dev, int groups, int64_t N, void* out_dev, int out_kind, void* stream);
 
-/* Low-rank adapters, one id per row (per_row 1): out = y + scale[g] (x down[g]^T) up[g]^T, in three products.
- * _shrink: planes[p] = scale[g] * x[order[p]] . down[g]^T (scale NULL: ones), as two bf16 parts per value: columns
- * [0, padded) the rounded value, [padded, 2 padded) the rounded remainder, padded = rank rounded up to 16;
- * ep_hip_low_rank_planes_bytes bytes, 16-byte aligned. down: [groups][rank][K], K a multiple of 8, 16-byte aligned rows.
- * _expand: out[order[p]] = y[order[p]] + planes[p] . up[g]^T (bf16; y NULL: zero; rows of no group: y). up: [groups][N][rank].
- * _reduce: out[g][e][n] (or, transposed, out[g][n][e]; bf16, contiguous) = sum over the places of g of planes[p][e] q[order[p]][n]; q
- * 16-byte aligned, ldq a multiple of 8, the columns from width to the next multiple of 8 readable; workspace 16-byte aligned. */
-int ep_hip_low_rank_shrink(const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group, const float* scale_dev, void* planes_dev,
-                           const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t K, void* stream);
-int ep_hip_low_rank_expand(const void* planes_dev, const void* up_dev, int64_t ldu, int64_t up_group, const void* y_dev, int64_t ldy, void* out_dev, int64_t ldo,
-                           const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t N, void* stream);
-int ep_hip_low_rank_reduce(const void* planes_dev, const void* q_dev, int64_t ldq, void* out_dev, int transposed, const int32_t* order_dev, const int32_t* offsets_dev,
-                           int64_t entries, int groups, int64_t rank, int64_t width, void* workspace_dev, size_t workspace_bytes, void* stream);
-size_t ep_hip_low_rank_reduce_workspace(int64_t entries, int groups, int64_t rank, int64_t width);
+/* Low-rank adapters, one id per row (per_row 1): out[t] = y[t] + scale[g] (x[t] down[g]^T) up[g]^T for the rows of adapter g, y[t] for rows
+ * of none (bf16; scale NULL: ones; y NULL: zero). x: [entries][K] and down: [groups][rank][K] are read in whole 16-byte pieces:
+ * 16-byte aligned, rows a multiple of 8 elements apart, zero from K to the next multiple of 8. up: [groups][N][rank].
+ * planes_dev (ep_hip_low_rank_planes_bytes bytes, 16-byte aligned) receives the narrow rows scale[g] x[order[p]] down[g]^T in grouped
+ * order, as two bf16 parts per value: columns [0, padded) the rounded value, [padded, 2 padded) the rounded remainder, padded =
+ * rank rounded up to 16. The gradient of up reads them.
+ * _grad: any of grad_x [entries][K] (rows of no adapter zero), grad_down [groups][rank][K] and grad_up [groups][N][rank] (contiguous),
+ * each absent when NULL, from grad_dev, the output's gradient [entries][N], read in whole pieces as x is; up is needed for the
+ * first two, down for the first, x for the second, planes (of the forward) for the third. workspace: 256-byte aligned. */
 size_t ep_hip_low_rank_planes_bytes(int64_t entries, int64_t rank);
+int ep_hip_low_rank_update(const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group, const void* up_dev, int64_t ldu, int64_t up_group,
+                           const float* scale_dev, const void* y_dev, int64_t ldy, void* planes_dev, void* out_dev, int64_t ldo, const int32_t* order_dev,
+                           const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t K, int64_t N, void* stream);
+size_t ep_hip_low_rank_grad_workspace(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N);
+int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group,
+                                const void* up_dev, int64_t ldu, int64_t up_group, const float* scale_dev, const void* planes_dev, void* grad_x_dev, int64_t ldgx,
+                                void* grad_down_dev, void* grad_up_dev, const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank,
+                                int64_t K, int64_t N, void* workspace_dev, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -168,7 +168,7 @@ def test_entry_points_refuse_bad_arguments():
     """Every check below fails before anything is launched, so no device is needed; the addresses are never followed."""
     lib, at, odd = hip.library(), 4096, 4104
     call = lambda name, good, **bad: getattr(lib, name)(*[bad.get(key, value) for key, value in good])
-    sort = [("ids", at), ("id_bytes", 8), ("entries", 5000), ("groups", 4), ("per_row", 1), ("order", at), ("offsets", at), ("place", at), ("rows", None), ("work", at), ("room", 1 << 20), ("stream", None)]
+    sort = [("ids", at), ("id_bytes", 8), ("entries", 9000), ("groups", 4), ("per_row", 1), ("order", at), ("offsets", at), ("place", at), ("rows", None), ("work", at), ("room", 1 << 20), ("stream", None)]
     for bad in ({"ids": None}, {"id_bytes": 2}, {"entries": 0}, {"groups": 0}, {"per_row": 0}, {"order": None}, {"offsets": None}, {"place": None}, {"work": None}, {"room": 8}):
         assert call("ep_hip_group_rows", sort, **bad) == hip.EINVAL, bad
     for bad in ({"groups": 897}, {"entries": (1 << 30) + 1}):
@@ -196,18 +196,18 @@ def test_entry_points_refuse_bad_arguments():
     for bad in ({"dy": None}, {"lddy": 4}, {"groups": 0}, {"N": 0}, {"out": None}, {"kind": 7}):
         assert call("ep_hip_grouped_column_sums_bf16", sums, **bad) == hip.EINVAL, bad
 
-    shrink = [("x", at), ("ldx", 16), ("down", at), ("ldd", 16), ("group", 64), ("scale", None), ("planes", at), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4),
-              ("K", 16), ("stream", None)]
-    for bad in ({"x": odd}, {"down": None}, {"planes": odd}, {"order": None}, {"rank": 0}, {"rank": 4097}, {"K": 12}, {"ldx": 8}, {"group": 4}, {"entries": 0}):
-        assert call("ep_hip_low_rank_shrink", shrink, **bad) == hip.EINVAL, bad
-    expand = [("planes", at), ("up", at), ("ldu", 4), ("group", 64), ("y", at), ("ldy", 16), ("out", at), ("ldo", 16), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4),
-              ("N", 16), ("stream", None)]
-    for bad in ({"planes": None}, {"up": None}, {"out": None}, {"ldu": 3}, {"ldy": 8}, {"ldo": 8}, {"group": -1}, {"N": 0}, {"offsets": None}):
-        assert call("ep_hip_low_rank_expand", expand, **bad) == hip.EINVAL, bad
-    reduce = [("planes", at), ("q", at), ("ldq", 16), ("out", at), ("transposed", 0), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4), ("width", 16), ("work", at),
-              ("room", 1 << 30), ("stream", None)]
-    for bad in ({"planes": None}, {"q": None}, {"out": None}, {"ldq": 8}, {"ldq": 20}, {"rank": 0}, {"width": 0}, {"q": odd}, {"work": None}, {"room": 16}):
-        assert call("ep_hip_low_rank_reduce", reduce, **bad) == hip.EINVAL, bad
+    update = [("x", at), ("ldx", 16), ("down", at), ("ldd", 16), ("down_group", 64), ("up", at), ("ldu", 4), ("up_group", 64), ("scale", None), ("y", at), ("ldy", 16), ("planes", at), ("out", at),
+              ("ldo", 16), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4), ("K", 16), ("N", 16), ("stream", None)]
+    for bad in ({"x": odd}, {"x": None}, {"ldx": 12}, {"ldx": 8}, {"down": None}, {"ldd": 20}, {"down_group": 4}, {"down_group": -8}, {"up": None}, {"ldu": 3}, {"up_group": -1}, {"ldy": 8},
+                {"planes": odd}, {"planes": None}, {"out": None}, {"ldo": 8}, {"order": None}, {"offsets": None}, {"entries": 0}, {"groups": 0}, {"rank": 0}, {"rank": 4097}, {"K": 0}, {"N": 0},
+                {"N": 1 << 30}, {"K": 17}):
+        assert call("ep_hip_low_rank_update", update, **bad) == hip.EINVAL, bad
+    grad = [("grad", at), ("ldg", 16), ("x", at), ("ldx", 16), ("down", at), ("ldd", 16), ("down_group", 64), ("up", at), ("ldu", 4), ("up_group", 64), ("scale", None), ("planes", at),
+            ("gx", at), ("ldgx", 16), ("gd", at), ("gu", at), ("order", at), ("offsets", at), ("entries", 8), ("groups", 2), ("rank", 4), ("K", 16), ("N", 16), ("work", at), ("room", 1 << 30),
+            ("stream", None)]
+    for bad in ({"grad": odd}, {"grad": None}, {"ldg": 8}, {"ldg": 20}, {"x": None}, {"ldx": 8}, {"down": None}, {"ldd": 8}, {"up": None}, {"ldu": 3}, {"planes": None}, {"planes": odd}, {"ldgx": 8},
+                {"gx": None, "gd": None, "gu": None}, {"order": None}, {"entries": 0}, {"rank": 0}, {"work": None}, {"work": 128}, {"room": 64}):
+        assert call("ep_hip_low_rank_update_grad", grad, **bad) == hip.EINVAL, bad
 
     combine = [("y", at), ("kind", 0), ("ldy", 8), ("place", at), ("kept", at), ("weight", at), ("weight_kind", 2), ("per_row", 2), ("tokens", 4), ("width", 8), ("out", at), ("ldo", 8), ("stream", None)]
     for bad in ({"y": None}, {"kind": 1}, {"ldy": 4}, {"kept": None}, {"weight_kind": 1}, {"per_row": 0}, {"tokens": 0}, {"width": 0}, {"out": None}, {"ldo": 4}):

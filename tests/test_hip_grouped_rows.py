@@ -61,7 +61,8 @@ def _plain_places(ids, groups):
 
 
 @pytest.mark.parametrize("tokens,per_row,groups", [(1, 0, 1), (1, 8, 3), (63, 1, 2), (64, 0, 64), (65, 2, 65), (1000, 3, 7), (4096, 1, 100), (4097, 1, 5), (2049, 4, 896),
-                                                   (20001, 8, 128), (300000, 5, 33)])
+                                                   (20001, 8, 128), (300000, 5, 33), (1024, 0, 9), (1025, 0, 896), (4096, 2, 64), (8193, 0, 3), (8192, 2, 64), (1 << 20, 0, 17),
+                                                   ((1 << 20) + 1, 0, 2)])
 @pytest.mark.parametrize("kind", ["even", "padded", "one", "none", "outside", "skewed"])
 def test_group_rows(tokens, per_row, groups, kind):
     print("case", tokens, per_row, groups, kind, flush=True)
@@ -349,6 +350,28 @@ def test_low_rank_update_strided_misaligned_and_spoiled_rows():
         assert torch.equal(got, ep.low_rank_update(y, spoiled, down, up, plan))
     big = torch.randn(4, 70, 24, device="cuda").bfloat16()
     assert torch.equal(ep.low_rank_update(wide[:, :64], wide[:, :128], down, big[:, 3:67, 1:9], plan), ep.low_rank_update(wide[:, :64], wide[:, :128], down, big[:, 3:67, 1:9].contiguous(), plan))
+
+
+def test_dimensions_of_one_with_any_stride():
+    """torch leaves the stride of a dimension of size one free, and calls such a tensor contiguous."""
+    plan = ep.group_rows(torch.ones(1, dtype=torch.int64, device="cuda"), 3)
+    x, y = torch.randn(64, 1, device="cuda").bfloat16().t(), torch.randn(40, 1, device="cuda").bfloat16().t()
+    down, up = torch.randn(3, 64, 1, device="cuda").bfloat16().transpose(1, 2), torch.randn(3, 1, 40, device="cuda").bfloat16().transpose(1, 2)
+    weight, dout = torch.randn(3, 64, 1, device="cuda").bfloat16().transpose(1, 2), torch.randn(40, 1, device="cuda").bfloat16().t()
+    plain = lambda *tensors: [t.clone(memory_format=torch.contiguous_format).requires_grad_(True) for t in tensors]
+
+    def both(run, grad, *operands):
+        odd = [t.detach().requires_grad_(True) for t in operands]
+        got = run(*odd)
+        even = plain(*operands)
+        want = run(*even)
+        assert torch.equal(got, want)
+        for a, b in zip(torch.autograd.grad(got, odd, grad), torch.autograd.grad(want, even, grad.clone(memory_format=torch.contiguous_format))):
+            assert a.shape == b.shape and torch.equal(a, b)
+
+    both(lambda y, x, d, u: ep.low_rank_update(y, x, d, u, plan), dout, y, x, down, up)
+    both(lambda x, w, b: ep.grouped_linear(x, w, plan, b), dout[:, :1], x, weight, torch.randn(3, 1, device="cuda").bfloat16())
+    both(lambda y: ep.combine_rows(y, plan), dout, y)
 
 
 def test_empty_batches():
