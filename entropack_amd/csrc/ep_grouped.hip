@@ -45,12 +45,16 @@ static bool rows_in_pieces(const void* base, int64_t ld, int64_t K, int element_
   return reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld >= K && (ld * element_bytes) % 16 == 0 && (K * element_bytes) % 16 == 0;
 }
 
+static int current_compute_units(int& units) {
+  int device = 0;
+  EP_HIP_TRY(hipGetDevice(&device));
+  EP_HIP_TRY(hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device));
+  return EP_HIP_OK;
+}
+
 // `tile` rows and columns per block: the 128 x 128 kernel or the 256 x 256 one.
 template <bool INT8, int MODE, bool GATHER = true>
 static int launch_tile(TileArgs t, int64_t row_tiles, int tile, hipStream_t s) {
-  int device = 0;
-  EP_HIP_TRY(hipGetDevice(&device));
-  EP_HIP_TRY(hipDeviceGetAttribute(&t.compute_units, hipDeviceAttributeMultiprocessorCount, device));
   const int64_t blocks = tile == kWideTile ? wide_blocks(row_tiles, t.columns, t.compute_units) : row_tiles * ((t.columns + kTile - 1) / kTile);
   if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
@@ -67,10 +71,19 @@ static int launch_tile(TileArgs t, int64_t row_tiles, int tile, hipStream_t s) {
   return EP_HIP_OK;
 }
 
-static int tile_for(int64_t entries, int groups, int64_t columns) {
-  (void)columns;
-  return entries / groups >= 256 ? kWideTile : kTile;
+// Rows and columns per block of a product of grouped rows (forward, rows' gradient). The 256 x 256 tiles read each operand half
+// as often as the 128 x 128 ones, but want half the device's compute units busy, tiles at least half full, and an inner dimension of 2 KB that pays for
+// the longer ends of a tile. us, 128 and 256: 8 groups of 4096 x 4096, 192 rows per group 80 and 81, 256 130 and 110, 1024 332
+// and 283; 64 of 2048 x 1408, 96 rows 118 and 122, 128 rows 142 and 124, 512 rows 396 and 289. 8 groups, 1024 rows, inner 512
+// and 4096 columns: 58 and 62; inner 4096 and 512 columns (64 tiles): 66 and 72.
+static int product_tile(int64_t entries, int groups, int64_t columns, int64_t inner_bytes, int compute_units) {
+  const bool wide = entries / groups >= kWideTile / 2 && entries * columns / (kWideTile * kWideTile) >= compute_units / 2 && inner_bytes >= 2048;
+  return wide ? kWideTile : kTile;
 }
+
+// Of a weights' gradient, whose inner dimension is a group's rows. 8 groups of 4096 x 4096, 256 rows per group 136 and 159 us, 512
+// 209 and 220, 1024 357 and 339, 2048 594 and 557; 64 of 2048 x 1408, 512 rows 295 and 322, 1024 539 and 519.
+static int grad_weight_tile(int64_t entries, int groups) { return entries / groups >= 768 ? kWideTile : kTile; }
 
 template <bool INT8>
 static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
@@ -88,7 +101,8 @@ static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
   t.lda_bytes = a.ldx_bytes, t.ldb_bytes = a.ldw_bytes, t.group_b_bytes = a.group_bytes, t.ldy = a.ldy;
   t.entries = a.entries, t.groups = a.groups, t.x_rows = a.x_rows, t.out_kind = a.out_kind;
   t.columns = a.N, t.inner = static_cast<int>(a.k_bytes);
-  const int tile = tile_for(a.entries, a.groups, a.N);
+  if (const int status = current_compute_units(t.compute_units)) return status;
+  const int tile = product_tile(a.entries, a.groups, a.N, a.k_bytes, t.compute_units);
   return launch_tile<INT8, kForward>(t, most_row_tiles(a.entries, a.groups, tile), tile, s);
 }
 
@@ -137,7 +151,8 @@ int ep_hip_grouped_grad_rows_bf16(const void* dy_dev, int64_t lddy, const void* 
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldw * 2, t.group_b_bytes = w_group * 2, t.ldy = lddx;
   t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(entries), t.out_kind = out_kind;
   t.columns = static_cast<int>(K), t.inner = static_cast<int>(N * 2);
-  const int tile = tile_for(entries, groups, K);
+  if (const int status = current_compute_units(t.compute_units)) return status;
+  const int tile = product_tile(entries, groups, K, t.inner, t.compute_units);
   return launch_tile<false, kGradRows>(t, most_row_tiles(entries, groups, tile), tile, static_cast<hipStream_t>(stream));
 }
 
@@ -153,7 +168,8 @@ int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldx * 2, t.ldy = lddw, t.group_y = dw_group;
   t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(x_rows), t.out_kind = out_kind;
   t.rows = static_cast<int>(N), t.columns = static_cast<int>(K);
-  const int tile = tile_for(entries, groups, K);
+  if (const int status = current_compute_units(t.compute_units)) return status;
+  const int tile = grad_weight_tile(entries, groups);
   const int64_t row_tiles = static_cast<int64_t>(groups) * ((N + tile - 1) / tile);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return rows_dev != nullptr ? launch_tile<false, kGradWeight, true>(t, row_tiles, tile, s) : launch_tile<false, kGradWeight, false>(t, row_tiles, tile, s);

@@ -74,6 +74,12 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ off
   return {groups, static_cast<int>(first), static_cast<int>(left < tile_rows ? left : tile_rows), tile - before};
 }
 
+// LDS accesses before it, of any lane of this wave, come before those after it.
+__device__ __forceinline__ void order_in_wave() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // How many tiles there are, those of no group included.
 __device__ __forceinline__ int64_t count_row_tiles(const int32_t* __restrict__ offsets, int groups, int entries, int tile_rows) {
   const int lane = threadIdx.x & 63;
@@ -178,7 +184,7 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
 #pragma unroll
     for (int i = 0; i < 4 * NT; ++i) *reinterpret_cast<uint4*>(staged_at(16 * MT + 4 * i + load_row, load_at)) = held_w[i];
     if (kb + stride < a.k_bytes) fetch(kb + stride);
-    __builtin_amdgcn_wave_barrier();
+    order_in_wave();
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       Frag fx[MT], fw[NT];
@@ -194,7 +200,7 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
           else acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[t], fw[j], acc[t][j], 0, 0, 0);
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    order_in_wave();
   }
   __syncthreads();
   // Register i of lane l holds row 4 (l / 16) + i and column l % 16 of its 16 x 16 tile.

@@ -29,12 +29,6 @@ __device__ __forceinline__ uint64_t lanes_with_my_key(int key, int key_bits, uin
   return same;
 }
 
-// LDS accesses before it, of any lane of this wave, come before those after it.
-__device__ __forceinline__ void order_in_wave() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // counts[key] (LDS, this wave's row, cleared before) += this wave's entries [first, last).
 template <typename Id>
 __device__ __forceinline__ void count_entries(const Id* __restrict__ ids, int64_t first, int64_t last, int groups, int key_bits, int* counts) {

@@ -311,7 +311,8 @@ static int shrink(const Grouping& g, const void* x, int64_t ldx, const void* dow
   a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = 2 * padded_rank(rank);
   a.entries = static_cast<int>(g.entries), a.groups = g.groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(g.entries), a.out_kind = kOutBF16;
   // All of a rank up to 64 in one block, so that x is read once. 4099 rows of 4096: rank 16 9.0 us (8 waves 10.5; 500 rows 6.0 against
-  // 5.4), rank 64 16.1 us (32 ranks per block 19.2); 7993 rows, rank 32, 18.5 us (16 rows per block 19.6; reading x takes 10.6).
+  // 5.4), rank 64 16.1 us (32 ranks per block 19.2); 7993 rows, rank 32, 18.5 us (16 rows per block 19.6,
+  // 48 rows on 6 waves, which need one round of blocks instead of two, 19.8; reading x takes 10.6).
   if (rank > 32) return launch_stream_of<false, 2, 4, 4, true>(a, s);
   if (rank > 16) return launch_stream_of<false, 2, 2, 8, true>(a, s);
   return g.entries >= 2048 ? launch_stream_of<false, 1, 1, 4, true>(a, s) : launch_stream_of<false, 1, 1, 8, true>(a, s);
