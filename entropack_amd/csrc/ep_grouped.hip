@@ -8,23 +8,48 @@
 
 namespace ep {
 
-// Sums of a group's rows, column by column: a block takes 64 columns of one group, its four waves every fourth row.
-__global__ __launch_bounds__(256) void grouped_column_sums_kernel(const uint16_t* __restrict__ dy, int64_t lddy, const int32_t* __restrict__ offsets, int N,
-                                                                  void* __restrict__ out, int out_kind) {
-  __shared__ float sums[4][64];
-  const int column_tiles = (N + 63) / 64;
+// Sums of a group's rows, column by column: a block takes 128 columns of one group, a lane two of them, its sixteen waves every
+// sixteenth row each, eight rows under way at a time. The partial sums are added in a fixed order. Bound by reading dy where
+// the groups make enough blocks: 16384 rows of 4096, 8 groups, 21.8 us (134 MB, 6.2 TB/s); one group, 32 blocks, 121 us. Four waves
+// with one column per lane and one row under way took 154 and 1142 us; 72 rows of 1408 in 64 groups take 3.8 us (2.5 with those).
+constexpr int kSumWaves = 16, kSumColumns = 128, kSumTogether = 8;
+
+__global__ __launch_bounds__(64 * kSumWaves) void grouped_column_sums_kernel(const uint16_t* __restrict__ dy, int64_t lddy, const int32_t* __restrict__ offsets, int N,
+                                                                             void* __restrict__ out, int out_kind, int pairs) {
+  __shared__ float sums[kSumWaves][kSumColumns];
+  const int column_tiles = (N + kSumColumns - 1) / kSumColumns;
   const int group = static_cast<int>(blockIdx.x / column_tiles);
-  const int n = static_cast<int>(blockIdx.x % column_tiles) * 64 + (threadIdx.x & 63);
-  const int wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = static_cast<int>(blockIdx.x % column_tiles) * kSumColumns + 2 * lane;
   const int first = offsets[group], last = offsets[group + 1];
-  float sum = 0.0f;
-  if (n < N) {
-    for (int p = first + wave; p < last; p += 4) sum += __uint_as_float(static_cast<uint32_t>(dy[p * lddy + n]) << 16);
+  const uint16_t* column = dy + (n < N ? n : 0);
+  const bool second = n + 1 < N;
+  float low = 0.0f, high = 0.0f;
+  for (int p = first + wave; p < last; p += kSumWaves * kSumTogether) {
+    uint32_t held[kSumTogether];                 // rows past the last read it again and count as zero
+#pragma unroll
+    for (int i = 0; i < kSumTogether; ++i) {
+      const int row = p + i * kSumWaves;
+      const uint16_t* at = column + (row < last ? row : last - 1) * lddy;
+      held[i] = pairs ? *reinterpret_cast<const uint32_t*>(at) : at[0] | static_cast<uint32_t>(at[second ? 1 : 0]) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < kSumTogether; ++i) {
+      const bool counts = p + i * kSumWaves < last;
+      low += counts ? __uint_as_float(held[i] << 16) : 0.0f;
+      high += counts ? __uint_as_float(held[i] & 0xFFFF0000u) : 0.0f;
+    }
   }
-  sums[wave][threadIdx.x & 63] = sum;
+  sums[wave][2 * lane] = low;
+  sums[wave][2 * lane + 1] = high;
   __syncthreads();
-  if (wave == 0 && n < N)
-    store_out(out, out_kind, static_cast<int64_t>(group) * N + n, (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]));
+  const int mine = static_cast<int>(blockIdx.x % column_tiles) * kSumColumns + static_cast<int>(threadIdx.x);
+  if (threadIdx.x < kSumColumns && mine < N) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSumWaves; ++w) sum += sums[w][threadIdx.x];
+    store_out(out, out_kind, static_cast<int64_t>(group) * N + mine, sum);
+  }
 }
 
 // ---- checks that every entry point makes --------------------------------------------------------------------------------------
@@ -179,9 +204,10 @@ int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int3
   using namespace ep;
   if (dy_dev == nullptr || offsets_dev == nullptr || out_dev == nullptr || groups <= 0 || N <= 0 || N > 0x7FFFFFFF / groups || lddy < N || !kind_valid(out_kind))
     return EP_HIP_EINVAL;
-  const int64_t blocks = groups * ((N + 63) / 64);
-  hipLaunchKernelGGL(grouped_column_sums_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const uint16_t*>(dy_dev), lddy, offsets_dev, static_cast<int>(N), out_dev, out_kind);
+  const int64_t blocks = groups * ((N + kSumColumns - 1) / kSumColumns);
+  const bool pairs = reinterpret_cast<uintptr_t>(dy_dev) % 4 == 0 && lddy % 2 == 0 && N % 2 == 0;
+  hipLaunchKernelGGL(grouped_column_sums_kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kSumWaves), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const uint16_t*>(dy_dev), lddy, offsets_dev, static_cast<int>(N), out_dev, out_kind, pairs ? 1 : 0);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;
 }
