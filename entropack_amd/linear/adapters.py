@@ -10,12 +10,13 @@ from __future__ import annotations
 import torch
 
 from ..backends import hip as _hip
-from .groups import RowGroups, device_of, matrix, rows_of
+from .groups import RowGroups, device_of, first_order, matrix, rows_of
 from .linear import CompressedLinear
 
 
-def _update(y, x, down, up, scale, groups: RowGroups) -> tuple[torch.Tensor, torch.Tensor]:
-    """The updated rows, and the narrow rows between the two products (two bf16 parts of the rank rounded up to 16 each)."""
+def _update(y, x, down, up, scale, groups: RowGroups):
+    """The updated rows; the narrow rows between the two products (two bf16 parts of the rank rounded up to 16 each); x, down and
+    up as the kernels read them."""
     rank, outer = up.shape[2], up.shape[1]
     planes = torch.empty(groups.entries, 2 * (-(-rank // 16) * 16), dtype=torch.bfloat16, device=x.device)
     out = torch.empty(groups.entries, outer, dtype=torch.bfloat16, device=x.device)
@@ -24,37 +25,38 @@ def _update(y, x, down, up, scale, groups: RowGroups) -> tuple[torch.Tensor, tor
                 rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0), wide.data_ptr(), wide.stride(1), wide.stride(0),
                 None if scale is None else scale.data_ptr(), base.data_ptr(), base.stride(0), planes.data_ptr(), out.data_ptr(), outer,
                 groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, x.shape[1], outer)
-    return out, planes
+    return out, planes, rows, narrow, wide
 
 
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, down, up, scale, groups):
-        out, planes = _update(y, x, down, up, scale, groups)
-        ctx.groups = groups
-        ctx.save_for_backward(x, down, up, scale, planes if ctx.needs_input_grad[3] else None)
+        out, planes, rows, narrow, wide = _update(y, x, down, up, scale, groups)
+        ctx.groups, ctx.inner = groups, x.shape[1]
+        ctx.save_for_backward(rows, narrow, wide, scale, planes if ctx.needs_input_grad[3] else None)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, grad):
-        x, down, up, scale, planes = ctx.saved_tensors
-        groups, (need_y, need_x, need_down, need_up) = ctx.groups, ctx.needs_input_grad[:4]
-        grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        grad_down = torch.empty(down.shape, dtype=down.dtype, device=x.device) if need_down else None
-        grad_up = torch.empty(up.shape, dtype=up.dtype, device=x.device) if need_up else None
-        if need_x or need_down or need_up:
-            inner, outer, rank = x.shape[1], up.shape[1], up.shape[2]
-            room = _hip.library().ep_hip_low_rank_grad_workspace(groups.entries, groups.groups, rank, inner, outer)
-            workspace = torch.empty(room, dtype=torch.uint8, device=x.device)
-            slope, rows, narrow, wide = matrix(grad, 8), matrix(x, 8), rows_of(down), rows_of(up)
-            _hip.launch("ep_hip_low_rank_update_grad", x.device,
-                        slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0),
-                        wide.data_ptr(), wide.stride(1), wide.stride(0), None if scale is None else scale.data_ptr(),
-                        None if planes is None else planes.data_ptr(), None if grad_x is None else grad_x.data_ptr(), inner,
-                        None if grad_down is None else grad_down.data_ptr(), None if grad_up is None else grad_up.data_ptr(),
-                        groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, groups.groups, rank, inner, outer,
-                        workspace.data_ptr(), room)
+        rows, narrow, wide, scale, planes = ctx.saved_tensors
+        groups, inner, device, (need_y, need_x, need_down, need_up) = ctx.groups, ctx.inner, grad.device, ctx.needs_input_grad[:4]
+        if not (need_x or need_down or need_up):
+            return grad, None, None, None, None, None
+        adapters, outer, rank = wide.shape
+        grad_x = torch.empty(groups.entries, inner, dtype=torch.bfloat16, device=device) if need_x else None
+        grad_down = torch.empty(adapters, rank, inner, dtype=torch.bfloat16, device=device) if need_down else None
+        grad_up = torch.empty(adapters, outer, rank, dtype=torch.bfloat16, device=device) if need_up else None
+        room = _hip.library().ep_hip_low_rank_grad_workspace(groups.entries, adapters, rank, inner, outer)
+        workspace = torch.empty(room, dtype=torch.uint8, device=device)
+        slope = matrix(grad, 8)
+        _hip.launch("ep_hip_low_rank_update_grad", device,
+                    slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), narrow.data_ptr(), narrow.stride(1), narrow.stride(0),
+                    wide.data_ptr(), wide.stride(1), wide.stride(0), None if scale is None else scale.data_ptr(),
+                    None if planes is None else planes.data_ptr(), None if grad_x is None else grad_x.data_ptr(), inner,
+                    None if grad_down is None else grad_down.data_ptr(), None if grad_up is None else grad_up.data_ptr(),
+                    groups.order.data_ptr(), groups.offsets.data_ptr(), groups.entries, adapters, rank, inner, outer,
+                    workspace.data_ptr(), room)
         return grad if need_y else None, grad_x, grad_down, grad_up, None, None
 
 

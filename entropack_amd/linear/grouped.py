@@ -17,7 +17,7 @@ import torch
 from ..backends import hip as _hip
 from ..compression import BatchDecompressor
 from . import kernels
-from .groups import RowGroups, device_of, matrix, rows_of, sum_entries
+from .groups import RowGroups, device_of, first_order, matrix, rows_of, sum_entries
 from .linear import CompressedINT8Linear, CompressedLinear
 
 
@@ -101,7 +101,7 @@ class _GroupedLinear(torch.autograd.Function):
         return _forward(x, weight, bias, groups, x_grouped)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, grad):
         x, weight = ctx.saved_tensors
         need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
@@ -179,7 +179,7 @@ class _CompressedGrouped(torch.autograd.Function):
         return layer._product(x.detach(), groups, x_grouped)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, grad):
         return _grad_rows(grad, ctx.layer.dequantize(grad.device).to(grad.dtype), ctx.groups, ctx.x_grouped), None, None, None
 

@@ -12,6 +12,7 @@ live meanwhile (torch ties a leaf's gradient accumulation to the stream it was f
 from __future__ import annotations
 
 import dataclasses
+import functools
 
 import torch
 
@@ -60,6 +61,16 @@ def rows_of(tensor: torch.Tensor) -> torch.Tensor:
         fits = fits and tensor.stride(dim) >= least
         least = tensor.stride(dim) * (tensor.shape[dim] - 1) + least
     return tensor if fits else tensor.clone(memory_format=torch.contiguous_format)
+
+
+def first_order(backward):
+    """`once_differentiable` where a graph of the gradients is asked for, without its two context managers where none is (3 us)."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 @dataclasses.dataclass(frozen=True, eq=False)
@@ -160,7 +171,7 @@ class _CombineRows(torch.autograd.Function):
         return _combine(y, weight, groups)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, grad):
         y, weight = ctx.saved_tensors
         groups, (need_y, need_weight, _) = ctx.groups, ctx.needs_input_grad
