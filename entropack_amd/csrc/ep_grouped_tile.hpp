@@ -90,6 +90,7 @@ __device__ __forceinline__ void store_wave_part(const TileArgs& g, Acc (&acc)[NI
         slab[slab_at(row, 32 * j + (lane & 31))] = v;
       }
     }
+    order_in_wave();
     if (!wide) {
 #pragma unroll 1
       for (int at = lane; at < 32 * kWidth; at += 64) {
@@ -132,6 +133,7 @@ __device__ __forceinline__ void store_wave_part(const TileArgs& g, Acc (&acc)[NI
         }
       }
     }
+    order_in_wave();                                        // the slab is free again
   }
 }
 

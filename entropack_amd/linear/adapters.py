@@ -72,7 +72,7 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         scale: f32 [adapters] or None for ones; it gets no gradient.
 
     Sums are f32; the narrow rows between the two products are kept in 16 bits of significand; the result is rounded to
-    bf16 once. Differentiable in y, x, down and up.
+    bf16 once. An infinity or NaN in a row's adapter makes that row's results NaN where it reaches them. Differentiable in y, x, down and up.
     """
     if not isinstance(groups, RowGroups):
         raise TypeError(f"low_rank_update takes the plan that group_rows returns, got {type(groups).__name__}")

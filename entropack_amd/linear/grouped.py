@@ -190,7 +190,8 @@ class CompressedGroupedLinear(torch.nn.Module):
     `experts`: `CompressedLinear` layers (bf16 containers) or `CompressedINT8Linear` layers, one class, one shape, with
     biases in all of them or in none. They stay ordinary submodules: `state_dict` holds `experts.<i>.weight.entropack_quant_state`
     and so on. A forward decodes all experts (in one pass when their weights are `lattice_rans` containers), then runs
-    `grouped_linear` or, for int8 experts, the row quantiser and `grouped_int8_linear`. Differentiable in x.
+    `grouped_linear` or, for int8 experts, the row quantiser and `grouped_int8_linear`. Differentiable in x. The first forward
+    plans the decode, which copies to the device: run one before capturing a graph.
     """
 
     def __init__(self, experts):
@@ -222,6 +223,10 @@ class CompressedGroupedLinear(torch.nn.Module):
         """Compresses one `torch.nn.Linear` per expert; keyword arguments go to the layers' `from_linear`."""
         layer_class = CompressedINT8Linear if int8 else CompressedLinear
         return cls([layer_class.from_linear(linear, **kwargs) for linear in linears])
+
+    def __getstate__(self):
+        # A decode plan holds addresses of this object's containers: a copy makes its own.
+        return {**self.__dict__, "_decoder": None}
 
     @property
     def groups(self) -> int:

@@ -5,6 +5,7 @@ Tolerances. Products of two bf16 numbers are exact in f32; a sum of K of them in
 round), and the one rounding to bf16 by half a step, 2^-8 of the value. `_bound` is that. Where a second product follows, the
 bound of the first is carried through the magnitudes; the two-part narrow rows of the adapters add 2^-16.
 """
+import copy
 import pytest
 import torch
 
@@ -544,3 +545,45 @@ def test_another_stream_and_a_replayed_graph():
         got = [t.clone() for t in held]
         assert all(torch.equal(a, b) for a, b in zip(got, step(x, ids, share))), replay
         assert torch.isfinite(torch.randn(1 << 20, device="cuda").sum()).item()
+
+
+def test_layers_copied_captured_and_used_on_two_streams_at_once():
+    experts, inner, outer, tokens = 3, 256, 192, 33
+    config = ep.EntroPackLossyConfig(target_bpp=4.0)
+    mixture = ep.CompressedGroupedLinear.from_linears([_dense(outer, inner, e) for e in range(experts)], config=config).cuda()
+    adapted = ep.AdaptedLinear(ep.CompressedLinear.from_linear(_dense(outer, inner, 7), config=config).cuda(), experts, 8).cuda()
+    adapted.set_adapter(1, torch.randn(8, inner) * 0.1, torch.randn(outer, 8) * 0.1)
+    x, ids = torch.randn(tokens, inner, device="cuda").bfloat16(), _ids(tokens, 0, experts, "padded")
+
+    def run(mixture, adapted, x, ids):
+        plan = ep.group_rows(ids, experts)
+        return ep.combine_rows(mixture(x, plan), plan), adapted(x, plan)
+
+    with torch.no_grad():
+        want = run(mixture, adapted, x, ids)
+        twins = copy.deepcopy(mixture), copy.deepcopy(adapted)
+        assert twins[0]._decoder is None and mixture._decoder is not None
+        assert all(torch.equal(a, b) for a, b in zip(run(*twins, x, ids), want))
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = []
+        for turn in range(6):
+            with torch.cuda.stream(streams[turn % 2]):
+                got.append(run(mixture, adapted, x, ids))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for result in got for a, b in zip(result, want))
+        fixed, fixed_ids = x.clone(), ids.clone()
+        graphs = []
+        for _ in range(2):                                # two graphs of the same layers
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                graphs.append((graph, run(mixture, adapted, fixed, fixed_ids)))
+        for seed in range(3):
+            fixed.copy_(torch.randn(tokens, inner, device="cuda"))
+            fixed_ids.copy_(_ids(tokens, 0, experts, "padded", seed))
+            expect = run(mixture, adapted, fixed, fixed_ids)
+            for graph, held in graphs:
+                graph.replay()
+            torch.cuda.synchronize()
+            for _, held in graphs:
+                assert all(torch.equal(a, b) for a, b in zip(held, expect)), seed
