@@ -20,7 +20,8 @@ from ..backends import hip as _hip
 
 MAX_GROUPS = 896                   # a thread per group and 64 KiB of LDS in the sorting kernel
 MAX_ENTRIES = 1 << 30
-_ROW_KINDS = {torch.bfloat16: 0, torch.float32: 2}
+_BF16, _F32 = 0, 2
+_ROW_KINDS = {torch.bfloat16: _BF16, torch.float32: _F32}
 
 
 def device_of(name: str, *tensors: torch.Tensor | None) -> torch.device:
@@ -42,9 +43,12 @@ def matrix(tensor: torch.Tensor, pieces: int) -> torch.Tensor:
     """`tensor` ([.., columns]) as the kernels read it: columns contiguous, rows and groups whole numbers of 16 bytes apart and
     not overlapping, the first row 16-byte aligned. Rows of a number of columns that is no multiple of `pieces` are padded
     with zeros. A tensor that lies so already is returned as it is; anything else is copied."""
-    columns = tensor.shape[-1]
+    shape = tensor.shape
+    columns = shape[-1]
     if columns % pieces:
         return torch.nn.functional.pad(tensor, (0, pieces - columns % pieces))
+    if 1 not in shape and tensor.is_contiguous():                # the usual case by one call; a dimension of one may have any stride
+        return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone(memory_format=torch.contiguous_format)
     fits = tensor.stride(-1) == 1 and tensor.data_ptr() % 16 == 0
     least = columns
     for dim in range(tensor.dim() - 2, -1, -1):
@@ -55,6 +59,8 @@ def matrix(tensor: torch.Tensor, pieces: int) -> torch.Tensor:
 
 def rows_of(tensor: torch.Tensor) -> torch.Tensor:
     """`tensor` ([.., columns]) for kernels that take any address: columns contiguous, rows and groups not overlapping."""
+    if 1 not in tensor.shape and tensor.is_contiguous():
+        return tensor
     fits = tensor.stride(-1) == 1
     least = tensor.shape[-1]
     for dim in range(tensor.dim() - 2, -1, -1):
@@ -151,38 +157,42 @@ def sum_entries(rows: torch.Tensor, tokens: int, per_row: int) -> torch.Tensor:
     return out
 
 
-def _combine(y, weight, groups: RowGroups) -> torch.Tensor:
+def _combine(y, weight, groups: RowGroups):
+    """The tokens' sums; y and the weights as the kernels read them."""
     rows = rows_of(y)
     ready = None if weight is None else weight.contiguous()
-    out = torch.empty(groups.tokens, y.shape[1], dtype=torch.bfloat16, device=y.device)
+    width = y.shape[1]
+    out = torch.empty(groups.tokens, width, dtype=torch.bfloat16, device=y.device)
     if out.numel():
         _hip.launch("ep_hip_combine_rows", y.device,
-                    rows.data_ptr(), _ROW_KINDS[torch.bfloat16], rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
+                    rows.data_ptr(), _BF16, rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
                     None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
-                    groups.tokens, rows.shape[1], out.data_ptr(), out.stride(0))
-    return out
+                    groups.tokens, width, out.data_ptr(), width)
+    return out, rows, ready
 
 
 class _CombineRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weight, groups):
+        out, rows, ready = _combine(y, weight, groups)
         ctx.groups = groups
-        ctx.save_for_backward(y, weight)
-        return _combine(y, weight, groups)
+        ctx.save_for_backward(rows, ready)
+        return out
 
     @staticmethod
     @first_order
     def backward(ctx, grad):
-        y, weight = ctx.saved_tensors
+        rows, ready = ctx.saved_tensors
         groups, (need_y, need_weight, _) = ctx.groups, ctx.needs_input_grad
-        grad_y = torch.empty_like(y, memory_format=torch.contiguous_format) if need_y else None
-        grad_weight = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_weight else None
-        if y.numel():
-            rows, ready, slope = rows_of(y), None if weight is None else weight.contiguous(), rows_of(grad)
-            _hip.launch("ep_hip_combine_rows_grad", y.device,
+        entries, width = rows.shape
+        grad_y = torch.empty(entries, width, dtype=torch.bfloat16, device=grad.device) if need_y else None
+        grad_weight = torch.empty(ready.shape, dtype=ready.dtype, device=grad.device) if need_weight else None
+        if entries and width:
+            slope = rows_of(grad)
+            _hip.launch("ep_hip_combine_rows_grad", grad.device,
                         slope.data_ptr(), slope.stride(0), rows.data_ptr(), rows.stride(0), groups.place.data_ptr(), kept_rows(groups),
                         None if ready is None else ready.data_ptr(), 0 if ready is None else _ROW_KINDS[ready.dtype], groups.per_row,
-                        groups.tokens, rows.shape[1], None if grad_y is None else grad_y.data_ptr(), rows.shape[1],
+                        groups.tokens, width, None if grad_y is None else grad_y.data_ptr(), width,
                         None if grad_weight is None else grad_weight.data_ptr())
         elif grad_weight is not None:
             grad_weight.zero_()
@@ -214,7 +224,7 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weight: torch.Tensor | None
     device_of("combine_rows", y, groups.order, weight)
     if torch.is_grad_enabled() and (y.requires_grad or (weight is not None and weight.requires_grad)):
         return _CombineRows.apply(y, weight, groups)
-    return _combine(y, weight, groups)
+    return _combine(y, weight, groups)[0]
 
 
 __all__ = ["RowGroups", "combine_rows", "group_rows"]
