@@ -587,3 +587,79 @@ def test_layers_copied_captured_and_used_on_two_streams_at_once():
             torch.cuda.synchronize()
             for _, held in graphs:
                 assert all(torch.equal(a, b) for a, b in zip(held, expect)), seed
+
+
+def test_any_subset_of_gradients_and_none_of_second_order():
+    groups, tokens, inner, outer, rank = 3, 50, 72, 40, 5
+    source = torch.Generator(device="cuda").manual_seed(5)
+    randn = lambda *shape: torch.randn(*shape, device="cuda", generator=source).bfloat16()
+    one, two = ep.group_rows(_ids(tokens, 0, groups, "padded"), groups), ep.group_rows(_ids(tokens, 2, groups, "padded"), groups)
+    share = torch.rand(tokens, 2, device="cuda", generator=source)
+    cases = [(lambda y, x, d, u: ep.low_rank_update(y, x, d, u, one), (randn(tokens, outer), randn(tokens, inner), randn(groups, rank, inner), randn(groups, outer, rank))),
+             (lambda x, w, b: ep.grouped_linear(x, w, two, b), (randn(tokens, inner), randn(groups, outer, inner), randn(groups, outer))),
+             (lambda y, w: ep.combine_rows(y, two, w), (randn(two.entries, outer), share)), (lambda y, w: ep.combine_rows(y, two, w), (randn(two.entries, outer), share.bfloat16()))]
+    for run, operands in cases:
+        full = [t.clone().requires_grad_(True) for t in operands]
+        out = run(*full)
+        dout = randn(*out.shape)
+        want = torch.autograd.grad(out, full, dout)
+        for chosen in range(1, 1 << len(operands)):
+            leaves = [t.clone().requires_grad_(bool(chosen >> i & 1)) for i, t in enumerate(operands)]
+            asked = [leaf for leaf in leaves if leaf.requires_grad]
+            got = torch.autograd.grad(run(*leaves), asked, dout)
+            assert all(torch.equal(a, want[i]) for a, i in zip(got, [i for i in range(len(operands)) if chosen >> i & 1])), chosen
+        first = torch.autograd.grad(run(*full), full[0], dout.requires_grad_(True), create_graph=True)[0]
+        assert torch.equal(first, want[0])
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
+
+
+def test_operands_past_two_to_the_31_elements():
+    """300000 rows of 8192: the last of them lie past 32 bits of elements. Few rows have a group; they are spread over the whole."""
+    tokens, wide, narrow, groups, rank = 300_000, 8192, 64, 3, 16
+    rows = torch.tensor([0, 1, 70_000, 140_001, 262_143, 262_144, 262_145, 299_998, 299_999], device="cuda")
+    ids = torch.full((tokens,), -1, dtype=torch.int64, device="cuda")
+    ids[rows] = torch.arange(len(rows), device="cuda") % groups
+    plan = ep.group_rows(ids, groups)
+    x = torch.zeros(tokens, wide, dtype=torch.bfloat16, device="cuda")
+    x[rows] = torch.randn(len(rows), wide, device="cuda").bfloat16()
+    x.requires_grad_(True)
+    weight = (torch.randn(groups, narrow, wide, device="cuda") * 0.05).bfloat16().requires_grad_(True)
+    kept, group, place = len(rows), ids[rows], plan.place.long()[rows]
+    y = ep.grouped_linear(x, weight, plan)
+    dy = torch.zeros_like(y)
+    dy[:kept] = torch.randn(kept, narrow, device="cuda").bfloat16()
+    gx, gw = torch.autograd.grad(y, (x, weight), dy)
+    # Against 64 bits: the mean rows per group choose the kernel and with it the order of the sums, so that the same rows in a small
+    # batch need not give the same bits.
+    xd, wd, dyd = x.detach()[rows].double(), weight.detach().double()[group], dy[place].double()
+    times = lambda a, b: (a.unsqueeze(1) @ b).squeeze(1)
+    want, size = times(xd, wd.transpose(1, 2).contiguous()), times(xd.abs(), wd.abs().transpose(1, 2).contiguous())
+    _within(y[place], want, _bound(want, size, wide))
+    _within(gx[rows], times(dyd, wd), _bound(times(dyd, wd), times(dyd.abs(), wd.abs()), narrow))
+    for g in range(groups):
+        mine = group == g
+        _within(gw[g], dyd[mine].t() @ xd[mine], _bound(dyd[mine].t() @ xd[mine], dyd[mine].abs().t() @ xd[mine].abs(), kept))
+    assert y[kept:].eq(0).all()
+    assert gx[:70_000][2:].eq(0).all() and gx[262_146:299_998].eq(0).all()
+    del gx, y, dy
+
+    down, up = (torch.randn(groups, rank, narrow, device="cuda") * 0.1).bfloat16(), torch.randn(groups, wide, rank, device="cuda").bfloat16()
+    thin = torch.randn(tokens, narrow, device="cuda").bfloat16()
+    with torch.no_grad():
+        out = ep.low_rank_update(x, thin, down, up, plan)
+        hidden, hidden_size = times(thin[rows].double(), down.double()[group].transpose(1, 2)), times(thin[rows].double().abs(), down.double()[group].abs().transpose(1, 2))
+        u = up.double()[group].transpose(1, 2)
+        want = x[rows].double() + times(hidden, u)
+        # the narrow sums' own error and their two parts' 2^-16, carried through |up|, besides the second product's
+        carried = times(narrow * STEP_F32 * hidden_size + 2.0 ** -16 * hidden.abs(), u.abs()) * 1.01
+        _within(out[rows], want, _bound(want, x[rows].double().abs() + times(hidden.abs(), u.abs()), 2 * rank + 1) + carried)
+        out[rows] = x[rows]
+        assert torch.equal(out, x)
+        del out
+        back = ep.low_rank_update(thin, x, torch.ones(groups, 1, wide, device="cuda").bfloat16(), torch.ones(groups, narrow, 1, device="cuda").bfloat16(), plan)
+        sums = x[rows].double().sum(1, keepdim=True)
+        want = thin[rows].double() + sums
+        _within(back[rows], want, _bound(want, x[rows].double().abs().sum(1, keepdim=True) + thin[rows].double().abs(), wide + 3) + 2.0 ** -16 * 1.01 * sums.abs())
+        combined = ep.combine_rows(x, plan)                  # here x holds places: those of a group are the first
+        assert torch.equal(combined[rows], x[plan.place.long()[rows]]) and combined[2:70_000].eq(0).all()
