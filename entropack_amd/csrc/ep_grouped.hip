@@ -1,8 +1,8 @@
 // Products of grouped rows with the weight of their group (a mixture's experts), and their gradients.
 //
-//   y[p]  = x[rows[p]] . w[g]^T (+ bias[g])            few rows per group: grouped_stream_kernel (ep_grouped.hpp), else grouped_tile_kernel
-//   dx[p] = dy[p] . w[g]                                    grouped_tile_kernel (ep_grouped_tile.hpp)
-//   dw[g] = sum_p dy[p]^T x[rows[p]]                        grouped_tile_kernel
+//   y[p]  = x[rows[p]] . w[g]^T (+ bias[g])                 few rows per group: grouped_stream_kernel (ep_grouped.hpp), else tiles
+//   dx[p] = dy[p] . w[g]                                    tiles: grouped_tile_kernel, grouped_wide_kernel (ep_grouped_tile.hpp)
+//   dw[g] = sum_p dy[p]^T x[rows[p]]                        tiles
 //   db[g] = sum_p dy[p]                                     grouped_column_sums_kernel
 #include "ep_grouped_tile.hpp"
 
