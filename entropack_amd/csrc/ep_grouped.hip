@@ -110,6 +110,37 @@ static int product_tile(int64_t entries, int groups, int64_t columns, int64_t in
 // 209 and 220, 1024 357 and 339, 2048 594 and 557; 64 of 2048 x 1408, 512 rows 295 and 322, 1024 539 and 519.
 static int grad_weight_tile(int64_t entries, int groups) { return entries / groups >= 768 ? kWideTile : kTile; }
 
+// Places per chunk of a weights' gradient, 0 for a group's places at once. A tile takes 0.62 us per 64 places, however few tiles there
+// are: with fewer tiles than compute units and long groups the places are divided so that about 512 blocks run, at least 512
+// places each, and the chunks' f32 sums are added by a second kernel. us, at once and in chunks: 2 weights of 128 x 128, 32768
+// rows each, 316 and 18; of 512 x 512, 319 and 81; one of 2048 x 1024, 8192 rows, 85 and 61; 8 of 1024 x 512, 2048 rows, 37 and
+// 37; 8 of 512 x 512, 1024 rows, 19 and 30.
+static int grad_weight_chunk(int64_t entries, int groups, int64_t N, int64_t K) {
+  const int64_t tiles = groups * ((N + kTile - 1) / kTile) * ((K + kTile - 1) / kTile);
+  if (tiles >= 256 || entries / groups < 4096) return 0;
+  const int64_t chunk = entries * tiles / groups / 512;       // entries / groups places in 512 / tiles chunks
+  return static_cast<int>(chunk < 512 ? 512 : (chunk + 63) / 64 * 64);
+}
+
+// out[g] = the sum of g's chunks, in their order, rounded once: a thread per element.
+__global__ __launch_bounds__(256) void grouped_sum_chunks_kernel(const float* __restrict__ parts, int chunk, const int32_t* __restrict__ offsets, int N, int K,
+                                                                 void* __restrict__ out, int64_t ld, int64_t group_out, int out_kind, int blocks_per_group) {
+  const int group = static_cast<int>(blockIdx.x) / blocks_per_group, lane = threadIdx.x & 63;
+  int before = 0;
+  for (int g0 = 0; g0 < group; g0 += 64) {
+    const int g = g0 + lane;
+    before += __builtin_amdgcn_readlane(wave_inclusive_sum(g < group ? (offsets[g + 1] - offsets[g] + chunk - 1) / chunk : 0), 63);
+  }
+  const int chunks = (offsets[group + 1] - offsets[group] + chunk - 1) / chunk;
+  const int64_t size = static_cast<int64_t>(N) * K, at = static_cast<int64_t>(static_cast<int>(blockIdx.x) % blocks_per_group) * 256 + threadIdx.x;
+  if (at >= size) return;
+  const float* from = parts + before * size + at;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int c = 0; c < chunks; ++c) sum += from[c * size];
+  store_out(out, out_kind, group * group_out + at / K * ld + at % K, sum);
+}
+
 template <bool INT8>
 static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
   // Few rows per group: the weights' stream (MI355X, weights from memory). About one row per group: blocks of 16 weight rows; one token,
@@ -181,9 +212,16 @@ int ep_hip_grouped_grad_rows_bf16(const void* dy_dev, int64_t lddy, const void* 
   return launch_tile<false, kGradRows>(t, most_row_tiles(entries, groups, tile), tile, static_cast<hipStream_t>(stream));
 }
 
+size_t ep_hip_grouped_grad_weight_workspace(int64_t entries, int groups, int64_t N, int64_t K) {
+  using namespace ep;
+  if (entries <= 0 || groups <= 0 || !sizes_valid(N, K, groups)) return 0;
+  const int chunk = grad_weight_chunk(entries, groups, N, K);
+  return chunk == 0 ? 0 : static_cast<size_t>(most_chunks(entries, groups, chunk)) * static_cast<size_t>(N) * static_cast<size_t>(K) * 4;
+}
+
 int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void* x_dev, int64_t ldx, int64_t x_rows, void* dw_dev, int64_t lddw, int64_t dw_group,
                                     int out_kind, const int32_t* rows_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
-                                    int64_t K, void* stream) {
+                                    int64_t K, void* workspace_dev, size_t workspace_bytes, void* stream) {
   using namespace ep;
   if (dy_dev == nullptr || x_dev == nullptr || dw_dev == nullptr || !groups_valid(offsets_dev, entries, groups, rows_dev, x_rows)) return EP_HIP_EINVAL;
   if (!sizes_valid(N, K, groups) || !kind_valid(out_kind) || lddw < K || dw_group < 0) return EP_HIP_EINVAL;
@@ -193,10 +231,22 @@ int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void
   t.lda_bytes = lddy * 2, t.ldb_bytes = ldx * 2, t.ldy = lddw, t.group_y = dw_group;
   t.entries = static_cast<int>(entries), t.groups = groups, t.x_rows = static_cast<int>(x_rows), t.out_kind = out_kind;
   t.rows = static_cast<int>(N), t.columns = static_cast<int>(K);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int chunk = grad_weight_chunk(entries, groups, N, K)) {
+    if (workspace_dev == nullptr || reinterpret_cast<uintptr_t>(workspace_dev) % 16 != 0 || workspace_bytes < ep_hip_grouped_grad_weight_workspace(entries, groups, N, K))
+      return EP_HIP_EINVAL;
+    t.y = workspace_dev, t.ldy = K, t.group_y = N * K, t.out_kind = kOutF32, t.chunk = chunk;
+    const int64_t row_tiles = most_chunks(entries, groups, chunk) * ((N + kTile - 1) / kTile), per_group = (N * K + 255) / 256;
+    const int status = rows_dev != nullptr ? launch_tile<false, kGradWeight, true>(t, row_tiles, kTile, s) : launch_tile<false, kGradWeight, false>(t, row_tiles, kTile, s);
+    if (status != EP_HIP_OK) return status;
+    hipLaunchKernelGGL(grouped_sum_chunks_kernel, dim3(static_cast<unsigned>(groups * per_group)), dim3(256), 0, s, static_cast<const float*>(workspace_dev), chunk, offsets_dev,
+                       static_cast<int>(N), static_cast<int>(K), dw_dev, lddw, dw_group, out_kind, static_cast<int>(per_group));
+    EP_HIP_TRY(hipGetLastError());
+    return EP_HIP_OK;
+  }
   if (const int status = current_compute_units(t.compute_units)) return status;
   const int tile = grad_weight_tile(entries, groups);
   const int64_t row_tiles = static_cast<int64_t>(groups) * ((N + tile - 1) / tile);
-  hipStream_t s = static_cast<hipStream_t>(stream);
   return rows_dev != nullptr ? launch_tile<false, kGradWeight, true>(t, row_tiles, tile, s) : launch_tile<false, kGradWeight, false>(t, row_tiles, tile, s);
 }
 

@@ -95,6 +95,9 @@ inline int64_t most_row_tiles(int64_t entries, int groups, int tile_rows) {
   return entries / tile_rows + parts;
 }
 
+// The most chunks of `chunk` places that `entries` places in `groups` groups make (places of no group are in none).
+inline int64_t most_chunks(int64_t entries, int groups, int chunk) { return entries / chunk + (groups < entries ? groups : entries); }
+
 // What a product on grouped rows is told. Place p reads row row_of[p] of x, or row p where row_of is null.
 struct GroupedArgs {
   const uint8_t* x;

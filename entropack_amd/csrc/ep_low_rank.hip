@@ -312,10 +312,6 @@ static int reduce_chunk(int64_t entries, int64_t rank, int64_t K, int64_t N) {
   return static_cast<int>(chunk < (1 << 30) ? chunk : 1 << 30);
 }
 
-static int64_t reduce_chunks(int64_t entries, int groups, int chunk) {       // the most there can be
-  return entries / chunk + (groups < entries ? groups : entries);
-}
-
 static int padded_rank(int64_t rank) { return static_cast<int>((rank + 15) / 16 * 16); }
 static int64_t whole_pieces(int64_t elements) { return (elements + 7) / 8 * 8; }
 static size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -382,7 +378,7 @@ static int expand(const Grouping& g, const void* planes, const void* up, int64_t
 
 // The chunks' sums of a gradient of so many columns.
 static size_t reduce_bytes(int64_t entries, int groups, int64_t rank, int chunk, int64_t width) {
-  return static_cast<size_t>(reduce_chunks(entries, groups, chunk)) * static_cast<size_t>(2 * padded_rank(rank)) * static_cast<size_t>(width) * 4;
+  return static_cast<size_t>(most_chunks(entries, groups, chunk)) * static_cast<size_t>(2 * padded_rank(rank)) * static_cast<size_t>(width) * 4;
 }
 
 // out[a][e][n] (transposed: out[a][n][e]) = sum over a's places of planes[p][e] q[order[p]][n]; rows of q readable to a whole number of pieces.
@@ -409,7 +405,7 @@ static int reduce(const Grouping& g, int64_t rank, int chunk, const Reduction* a
     t.entries = static_cast<int>(g.entries), t.groups = g.groups, t.x_rows = static_cast<int>(g.entries), t.out_kind = kOutF32;
     t.rows = 2 * padded, t.columns = static_cast<int>(r.width), t.chunk = chunk;
     sums[i] = {static_cast<const float*>(r.parts), static_cast<uint16_t*>(r.out), static_cast<int>(r.width), r.transposed ? 1 : 0};
-    blocks[i] = reduce_chunks(g.entries, g.groups, chunk) * ((t.rows + kTile - 1) / kTile) * ((r.width + kTile - 1) / kTile);
+    blocks[i] = most_chunks(g.entries, g.groups, chunk) * ((t.rows + kTile - 1) / kTile) * ((r.width + kTile - 1) / kTile);
     finish[i] = static_cast<int64_t>(g.groups) * (padded / 16) * ((r.width + 63) / 64);
   }
   if (blocks[0] + blocks[1] > 0x7FFFFFFF || finish[0] + finish[1] > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;

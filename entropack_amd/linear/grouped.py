@@ -74,10 +74,13 @@ def _grad_weight(grad, x, weight, groups: RowGroups, x_grouped: bool) -> torch.T
     dy, rows = matrix(grad, 8), matrix(x, 8)
     outer, inner = dy.shape[1], rows.shape[1]
     out = torch.empty(groups.groups, outer, inner, dtype=torch.bfloat16, device=grad.device)
+    room = _hip.library().ep_hip_grouped_grad_weight_workspace(groups.entries, groups.groups, outer, inner)
+    workspace = torch.empty(room, dtype=torch.uint8, device=grad.device) if room else None
     _hip.launch("ep_hip_grouped_grad_weight_bf16", grad.device,
                 dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), rows.shape[0], out.data_ptr(), inner, outer * inner,
                 _hip.FLOAT_KINDS[torch.bfloat16], None if x_grouped else groups.rows.data_ptr(),
-                groups.offsets.data_ptr(), groups.entries, groups.groups, outer, inner)
+                groups.offsets.data_ptr(), groups.entries, groups.groups, outer, inner,
+                None if workspace is None else workspace.data_ptr(), room)
     return out if tuple(out.shape) == tuple(weight.shape) else out[:, :weight.shape[1], :weight.shape[2]].contiguous()
 
 

@@ -454,12 +454,13 @@ int ep_hip_grouped_gemm_i8(const int8_t* x_dev, int64_t ldx, int64_t x_rows, con
 /* Gradients of ep_hip_grouped_gemm_bf16, dy in grouped order, rows 16-byte aligned.
  * _grad_rows (any N, the columns of dy from N to the next multiple of 8 readable and zero): row order[p] of dx (row p where order_dev is NULL) = dy[p] . w[g], zero for entries of no group.
  * _grad_weight (N a multiple of 8): dw[g] ([N][K], rows lddw and groups dw_group elements apart) = sum over the places of g of dy[p]^T x[rows[p]];
- * zero for a group without rows. _column_sums: out[g][n] = sum of dy[p][n] (the bias's gradient). */
+ * zero for a group without rows; few small weights with many rows each take a 16-byte aligned workspace (its size is 0 otherwise). _column_sums: out[g][n] = sum of dy[p][n] (the bias's gradient). */
 int ep_hip_grouped_grad_rows_bf16(const void* dy_dev, int64_t lddy, const void* w_dev, int64_t ldw, int64_t w_group, void* dx_dev, int64_t lddx, int out_kind,
                                   const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N, int64_t K, void* stream);
+size_t ep_hip_grouped_grad_weight_workspace(int64_t entries, int groups, int64_t N, int64_t K);
 int ep_hip_grouped_grad_weight_bf16(const void* dy_dev, int64_t lddy, const void* x_dev, int64_t ldx, int64_t x_rows, void* dw_dev, int64_t lddw, int64_t dw_group,
                                     int out_kind, const int32_t* rows_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t N,
-                                    int64_t K, void* stream);
+                                    int64_t K, void* workspace_dev, size_t workspace_bytes, void* stream);
 int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int32_t* offsets_dev, int groups, int64_t N, void* out_dev, int out_kind, void* stream);
 
 /* Low-rank adapters, one id per row (per_row 1): out[t] = y[t] + scale[g] (x[t] down[g]^T) up[g]^T for the rows of adapter g, y[t] for rows

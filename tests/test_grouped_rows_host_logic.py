@@ -189,8 +189,11 @@ def test_entry_points_refuse_bad_arguments():
     for bad in ({"dy": odd}, {"w": None}, {"dx": None}, {"lddx": 8}, {"N": 9}, {"K": 12}, {"lddy": 4}, {"offsets": None}):
         assert call("ep_hip_grouped_grad_rows_bf16", rows, **bad) == hip.EINVAL, bad
     weight = [("dy", at), ("lddy", 8), ("x", at), ("ldx", 16), ("x_rows", 8), ("dw", at), ("lddw", 16), ("dw_group", 128), ("kind", 0), ("rows", at), ("offsets", at),
-              ("entries", 8), ("groups", 2), ("N", 8), ("K", 16), ("stream", None)]
-    for bad in ({"dy": odd}, {"x": odd}, {"dw": None}, {"lddw": 8}, {"N": 4}, {"K": 12}, {"dw_group": -1}, {"rows": None, "x_rows": 7}):
+              ("entries", 8), ("groups", 2), ("N", 8), ("K", 16), ("work", None), ("room", 0), ("stream", None)]
+    long = {"entries": 10000, "x_rows": 10000}                     # two small weights, many rows: the sums of chunks take a workspace
+    room = lib.ep_hip_grouped_grad_weight_workspace(10000, 2, 8, 16)
+    assert room > 0 and lib.ep_hip_grouped_grad_weight_workspace(8, 2, 8, 16) == 0 and lib.ep_hip_grouped_grad_weight_workspace(1 << 20, 8, 4096, 4096) == 0
+    for bad in ({**long, "work": at, "room": room - 1}, {**long, "work": odd, "room": room}, {**long, "room": room}, {"dy": odd}, {"x": odd}, {"dw": None}, {"lddw": 8}, {"N": 4}, {"K": 12}, {"dw_group": -1}, {"rows": None, "x_rows": 7}):
         assert call("ep_hip_grouped_grad_weight_bf16", weight, **bad) == hip.EINVAL, bad
     sums = [("dy", at), ("lddy", 8), ("offsets", at), ("groups", 2), ("N", 8), ("out", at), ("kind", 0), ("stream", None)]
     for bad in ({"dy": None}, {"lddy": 4}, {"groups": 0}, {"N": 0}, {"out": None}, {"kind": 7}):

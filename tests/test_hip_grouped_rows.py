@@ -90,7 +90,8 @@ def test_group_rows_takes_strided_ids_wide_values_and_none_at_all():
 PRODUCTS = [(1, 2, 8, 264, 100, "even"), (1, 0, 1, 8, 1, "even"), (5, 4, 64, 512, 129, "padded"), (40, 2, 3, 72, 257, "even"), (33, 1, 4, 1024, 64, "one"),
             (7, 3, 5, 128, 40, "none"), (129, 2, 5, 320, 130, "outside"), (300, 2, 4, 136, 264, "skewed"), (1100, 2, 3, 200, 384, "padded"), (700, 0, 2, 1096, 520, "even"),
             (64, 8, 4, 33, 65, "even"), (513, 4, 6, 2048, 128, "skewed"), (260, 1, 896, 64, 72, "even"), (2100, 1, 1, 448, 1000, "one"),
-            (4100, 2, 6, 2064, 1041, "padded"), (2100, 2, 4, 2048, 2304, "even"), (4200, 0, 3, 1032, 2056, "one"), (4300, 2, 3, 1024, 2056, "even"), (5000, 2, 4, 2056, 2100, "skewed")]
+            (4100, 2, 6, 2064, 1041, "padded"), (2100, 2, 4, 2048, 2304, "even"), (4200, 0, 3, 1032, 2056, "one"), (4300, 2, 3, 1024, 2056, "even"), (5000, 2, 4, 2056, 2100, "skewed"),
+            (9000, 0, 2, 136, 72, "padded"), (7001, 2, 3, 128, 128, "skewed"), (5000, 2, 1, 264, 9, "outside"), (5000, 2, 2, 520, 264, "one")]
 
 
 def _product_operands(case, x_grouped, seed=3):
