@@ -125,9 +125,10 @@ __device__ __forceinline__ int source_row(const GroupedArgs& a, int place) {
 // fragments of the 16 x 16 matrix-core instructions want sixteen rows (lane l holds 16 bytes of row l % 16, at byte 16 (l / 16)
 // of a 64-byte step): the piece goes through LDS private to the wave, while the next one is on its way in registers, so that
 // there is no barrier in the loop. Loading the fragments straight from memory occupies the address path four times as long.
-// PLANES: the sums are multiplied with scale_x[group] and stored as two bf16 parts, the rounded value and the rounded
-// remainder, columns [0, padded) and [padded, 2 padded) of row p of y, padded = N rounded up to 16; columns from N on are 0.
-// The product that reads them then works on 16 bits of significand instead of 8, in the memory that f32 would take.
+// PLANES: the sums are multiplied with scale_x[group] and stored as three bf16 parts, the rounded value, the rounded remainder and what
+// then remains: 8 bits of significand each, so that the three add up to the f32 value exactly (above 2^-110, where the last part leaves
+// the range of bf16). Row p of y holds 64 columns for every 16 of N: 16 values, 16 remainders, 16 last parts and 16 zeros, which is how the
+// products that read it take them; columns from N to the next multiple of 16 are 0.
 template <bool INT8, int MT, int NT, int WAVES, bool PLANES>
 __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs a) {
   using Acc = typename std::conditional<INT8, i32x4, f32x4>::type;
@@ -225,12 +226,15 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
       const int padded = (a.N + 15) & ~15;
       if (n >= padded) continue;
       float v = n < a.N ? static_cast<float>(sum) : 0.0f;
-      if (a.scale_x != nullptr && n < a.N) v *= a.scale_x[tile.group];
-      uint16_t* out = static_cast<uint16_t*>(a.y) + place * a.ldy + n;
+      if (a.scale_x != nullptr && n < a.N) v = __fmul_rn(v, a.scale_x[tile.group]);      // rounded before it is divided into parts
+      uint16_t* out = static_cast<uint16_t*>(a.y) + place * a.ldy + 4 * (n & ~15) + (n & 15);
       const uint32_t high = bf16_bits_of(v);
-      const float rest = v - __uint_as_float(high << 16);
+      const float rest = (high & 0x7F80u) == 0x7F80u ? 0.0f : v - __uint_as_float(high << 16);      // an infinity has no remainder
+      const uint32_t middle = bf16_bits_of(rest);
       out[0] = static_cast<uint16_t>(high);
-      out[padded] = (high & 0x7F80u) == 0x7F80u ? 0 : static_cast<uint16_t>(bf16_bits_of(rest));    // an infinity has no remainder
+      out[16] = static_cast<uint16_t>(middle);
+      out[32] = static_cast<uint16_t>(bf16_bits_of(rest - __uint_as_float(middle << 16)));
+      out[48] = 0;
     } else if (n < a.N) {
       const bool has_bias = a.bias != nullptr;
       const float b = has_bias ? load_bias(a.bias, a.out_kind, tile.group * a.N + n) : 0.0f;

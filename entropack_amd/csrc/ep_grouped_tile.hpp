@@ -158,9 +158,11 @@ struct ColumnLoads {
   __device__ static int piece(int wave, int lane) { return (lane % (W / 8)) ^ ((first_inner(wave, lane) & 3) << 2); }
 };
 
+// FOLD (weights' gradient to f32): the rows of y are the narrow rows' three parts, 64 rows for 16 ranks as they lie in the planes, and are added
+// up here: y has a row per rank.
 // TAIL = false: the inner length is a whole number of rounds of two steps (and, in the rows' gradient, the columns a whole number of
 // tiles), so that no piece lies outside. GATHER: the weights' gradient with row_of (the other modes look at the pointer).
-template <bool INT8, int MODE, bool TAIL, bool GATHER, int TM, int TN, int STAGE>
+template <bool INT8, int MODE, bool TAIL, bool GATHER, int TM, int TN, bool FOLD = false, int STAGE>
 __device__ __forceinline__ void compute_tile(const TileArgs& g, const BlockTile& tile, uint8_t (&stage0)[STAGE], uint8_t (&stage1)[STAGE], int32_t* row_at, float* scale_at) {
   static_assert(!INT8 || MODE == kForward, "gradients are bf16");
   static_assert(STAGE >= (TM + TN) * 128, "a stage holds both operands' tiles");
@@ -346,6 +348,21 @@ __device__ __forceinline__ void compute_tile(const TileArgs& g, const BlockTile&
       k_step(stage1, stage0, step + 1);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);
+  }
+  if constexpr (FOLD) {
+    // A wave's 64 rows are one stretch of 16 ranks: values in registers 0 .. 7 of its first 32 x 32 tiles, remainders in 8 .. 15, last parts in
+    // 0 .. 7 of the second, all three of a rank and column in one lane.
+    static_assert(MODE == kGradWeight && TM == 128, "64 rows per wave");
+    if (m0 + 64 * wave_m >= g.rows) return;
+    float* const to = static_cast<float*>(g.y) + group * g.group_y + (m0 / 4 + 16 * wave_m) * g.ldy;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int n = n0 + (TN / 2) * wave_n + 32 * j + (lane & 31);
+      if (n >= g.columns) continue;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) to[(8 * (r / 4) + 4 * (lane >> 5) + r % 4) * g.ldy + n] = acc[0][j][r] + (acc[0][j][r + 8] + acc[1][j][r]);
+    }
+    return;
   }
   __syncthreads();                                          // every load has landed and every fragment is read: the stages are free
   static_assert(4 * 32 * (TN / 2) * 4 <= STAGE, "four slabs fit into a stage");

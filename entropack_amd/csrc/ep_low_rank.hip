@@ -4,15 +4,15 @@
 //   expand   out[order[p]] = y[order[p]] + planes[p] . up[a]^T   low_rank_expand_kernel, bound by reading y and writing out
 //   reduce   sum_p planes[p]^T q[order[p]]                     low_rank_reduce_kernel, low_rank_finish_kernel: the gradients of down (q = x, planes of the
 //                                                              output's gradient) and of up (q = the output's gradient)
-// The narrow rows in between ("planes") are kept as two bf16 parts, value and remainder, so that the second product loses
-// nothing that the output's own rounding would show: each rounding is off by at most 2^-8 of what it
-// rounds, so the two parts together by at most 2^-16 of the f32 value.
+// The narrow rows in between ("planes") are kept as three bf16 parts that add up to the f32 value exactly, so that the second product runs on
+// the bf16 matrix cores and loses nothing, also where y and the update cancel. (Two parts are off by up to 2^-16 of the value, which
+// the output's rounding hides only where nothing cancels.) A rank's three parts meet the same element of the other operand.
 #include "ep_grouped_tile.hpp"
 
 namespace ep {
 
 struct LowRankArgs {
-  const uint16_t* planes;          // [entries][2 padded]
+  const uint16_t* planes;          // [entries][4 padded]: for every 16 ranks 16 values, 16 remainders, 16 last parts, 16 zeros
   const uint16_t* up;              // [groups][N][rank]
   const uint16_t* y;               // [rows][N], or null for zero
   uint16_t* out;
@@ -55,8 +55,8 @@ __device__ __forceinline__ uint4 add_to_pieces(uint4 in, const f32x4& first, con
 
 // Few rows per adapter: a block takes 16 rows of one adapter and 256 columns, a wave 64 of them. The matrix cores are given the rows
 // of `up` as the left operand, ordered so that a lane ends up with two runs of 8 consecutive columns of its row (row m of tile j
-// is column 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4 of the 64). The inner dimension is [value | remainder], both against the
-// same `up`. There is no LDS and nothing to wait for but the loads: 61 rows of 48 adapters take 3.5 us.
+// is column 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4 of the 64). The inner dimension is [value | remainder] and [last part | zeros] of
+// 16 ranks, all against the same `up`. There is no LDS and nothing to wait for but the loads: 61 rows of 48 adapters take 3.5 us.
 template <bool PIECES, bool WIDE>
 __global__ __launch_bounds__(256) void low_rank_expand_kernel(LowRankArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -77,19 +77,21 @@ __global__ __launch_bounds__(256) void low_rank_expand_kernel(LowRankArgs a) {
   }
   f32x4 acc[4] = {};
   if (tile.group < a.groups) {
-    const uint16_t* planes = a.planes + (static_cast<int64_t>(tile.first) + (in_row < tile.rows ? in_row : tile.rows - 1)) * (2 * a.padded) + 8 * quarter;
+    const uint16_t* planes = a.planes + (static_cast<int64_t>(tile.first) + (in_row < tile.rows ? in_row : tile.rows - 1)) * (4 * a.padded) + 8 * quarter;
     const uint16_t* up[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = n0 + 32 * (j >> 1) + 8 * (in_row >> 2) + 4 * (j & 1) + (in_row & 3);
       up[j] = a.up + tile.group * a.up_group + (row < a.N ? row : a.N - 1) * a.ldu;
     }
-    for (int e0 = 0; e0 < 2 * a.padded; e0 += 32) {
-      const int e = e0 + 8 * quarter, in_up = e < a.padded ? e : e - a.padded;
-      const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + e0);
+    for (int e0 = 0; e0 < a.padded; e0 += 16) {
+      const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + 4 * e0);
+      const bf16x8 last = *reinterpret_cast<const bf16x8*>(planes + 4 * e0 + 32);
       bf16x8 fu[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fu[j] = __builtin_bit_cast(bf16x8, up_piece<PIECES>(up[j], in_up, a.rank));
+      for (int j = 0; j < 4; ++j) fu[j] = __builtin_bit_cast(bf16x8, up_piece<PIECES>(up[j], e0 + 8 * (quarter & 1), a.rank));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fu[j], last, acc[j], 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fu[j], fp, acc[j], 0, 0, 0);
     }
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
   f32x4 acc[8] = {};
   if (grouped) {
     const int plane_row = 16 * wave + in_row < tile.rows ? 16 * wave + in_row : tile.rows - 1;
-    const uint16_t* planes = a.planes + (static_cast<int64_t>(tile.first) + plane_row) * (2 * a.padded) + (quarter >> 1) * a.padded;
+    const uint16_t* planes = a.planes + (static_cast<int64_t>(tile.first) + plane_row) * (4 * a.padded) + 8 * quarter;
     const uint16_t* up = a.up + tile.group * a.up_group;
     for (int rank0 = 0; rank0 < a.padded; rank0 += STEP) {
       uint4 moved[kMoves];
@@ -169,13 +171,14 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
       }
       __syncthreads();
       const int ranks = a.padded - rank0 < STEP ? a.padded - rank0 : STEP;
-      // 32 of the inner dimension at a time: 16 ranks' values and remainders (quarters 0, 1 and 2, 3), both against the same `up`.
+      // 16 ranks at a time: values and remainders (quarters 0, 1 and 2, 3), then last parts and zeros, both against the same `up`.
       for (int e0 = 0; e0 < ranks; e0 += 16) {
-        const int e = e0 + 8 * (quarter & 1);
-        const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + rank0 + e);
+        const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + 4 * (rank0 + e0));
+        const bf16x8 last = *reinterpret_cast<const bf16x8*>(planes + 4 * (rank0 + e0) + 32);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bf16x8 fu = *reinterpret_cast<const bf16x8*>(up_tile + (16 * j + in_row) * kPitch + 2 * e);
+          const bf16x8 fu = *reinterpret_cast<const bf16x8*>(up_tile + (16 * j + in_row) * kPitch + 2 * (e0 + 8 * (quarter & 1)));
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(last, fu, acc[j], 0, 0, 0);
           acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp, fu, acc[j], 0, 0, 0);
         }
       }
@@ -200,8 +203,9 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
   }
 }
 
-// sum over a group's places of planes[p][e] q[order[p]][n] for all e < rank (value + remainder): out[g][e][n], or out[g][n][e] when
-// transposed. The products are the weights' gradient of ep_grouped_tile.hpp with the planes as left operand. They are bound by
+// sum over a group's places of planes[p][e] q[order[p]][n] for all e < rank: out[g][e][n], or out[g][n][e] when
+// transposed. The products are the weights' gradient of ep_grouped_tile.hpp with the planes as left operand, the three parts' sums folded
+// into one where the tile is stored. They are bound by
 // reading q, and the groups alone make too few tiles to fill the card, so the places of every group are divided into chunks, each
 // chunk writes its f32 sums to a matrix of its own, and this kernel adds a group's chunks in their order and rounds once.
 // A block takes 64 columns and 16 ranks of one group, a wave one of the ranks; bound by the latency of its loads: 36 chunks of rank 16
@@ -228,14 +232,13 @@ __global__ __launch_bounds__(1024) void low_rank_finish_kernel(Finish of_first, 
   for (int g = lane; g < group; g += 64) before += (offsets[g + 1] - offsets[g] + chunk - 1) / chunk;
   before = __builtin_amdgcn_readlane(wave_inclusive_sum(before), 63);
   const int chunks = (offsets[group + 1] - offsets[group] + chunk - 1) / chunk;
-  const int64_t matrix = static_cast<int64_t>(2 * padded) * width;
+  const int64_t matrix = static_cast<int64_t>(padded) * width;
   const int n = n0 + lane, e = e0 + wave;
   float sum = 0.0f;
   if (n < width) {
-    const float* high = f.parts + before * matrix + static_cast<int64_t>(e) * width + n;
-    const float* low = high + static_cast<int64_t>(padded) * width;
+    const float* from = f.parts + before * matrix + static_cast<int64_t>(e) * width + n;
 #pragma unroll 4
-    for (int c = 0; c < chunks; ++c) sum += high[c * matrix] + low[c * matrix];
+    for (int c = 0; c < chunks; ++c) sum += from[c * matrix];
   }
   const uint16_t bits = static_cast<uint16_t>(bf16_bits_of(sum));
   if (!f.transposed) {
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void low_rank_reduce_kernel(TileAr
   const TileArgs g = second ? of_second : of_first;
   BlockTile tile;
   if (!find_block_tile<kGradWeight>(g, static_cast<int>(blockIdx.x) - (second ? first_blocks : 0), kTile, tile)) return;
-  compute_tile<false, kGradWeight, true, true, kTile, kTile>(g, tile, stage0, stage1, row_at, scale_at);
+  compute_tile<false, kGradWeight, true, true, kTile, kTile, true>(g, tile, stage0, stage1, row_at, scale_at);
 }
 
 // Both transposes that the gradients need, [groups][rows][columns] to [groups][columns][out_rows] with zeros in rows .. out_rows: 64 x 64
@@ -305,7 +308,7 @@ __global__ __launch_bounds__(256) void low_rank_transpose_kernel(Transpose first
 
 // Places per chunk: about 1024 tiles in all, both gradients', at least 128 places each (a chunk of fewer does not outlast its own prologue).
 static int reduce_chunk(int64_t entries, int64_t rank, int64_t K, int64_t N) {
-  const int64_t tiles = ((K + kTile - 1) / kTile + (N + kTile - 1) / kTile) * (((rank + 15) / 16 * 32 + kTile - 1) / kTile);
+  const int64_t tiles = ((K + kTile - 1) / kTile + (N + kTile - 1) / kTile) * (((rank + 15) / 16 * 64 + kTile - 1) / kTile);
   const int64_t chunks = tiles >= 1024 ? 1 : 1024 / tiles;
   int64_t chunk = (entries + chunks - 1) / chunks;
   chunk = chunk < 128 ? 128 : (chunk + 63) / 64 * 64;
@@ -315,7 +318,7 @@ static int reduce_chunk(int64_t entries, int64_t rank, int64_t K, int64_t N) {
 static int padded_rank(int64_t rank) { return static_cast<int>((rank + 15) / 16 * 16); }
 static int64_t whole_pieces(int64_t elements) { return (elements + 7) / 8 * 8; }
 static size_t whole_lines(size_t bytes) { return (bytes + 255) / 256 * 256; }
-static size_t planes_bytes(int64_t entries, int64_t rank) { return static_cast<size_t>(entries) * static_cast<size_t>(padded_rank(rank)) * 4; }
+static size_t planes_bytes(int64_t entries, int64_t rank) { return static_cast<size_t>(entries) * static_cast<size_t>(padded_rank(rank)) * 8; }
 
 // The adapters and the rows they are for.
 struct Grouping {
@@ -330,7 +333,7 @@ static int shrink(const Grouping& g, const void* x, int64_t ldx, const void* dow
                   hipStream_t s) {
   GroupedArgs a = {};
   a.x = static_cast<const uint8_t*>(x), a.w = static_cast<const uint8_t*>(down), a.scale_x = scale, a.y = planes, a.row_of = g.order, a.offsets = g.offsets;
-  a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = 2 * padded_rank(rank);
+  a.ldx_bytes = ldx * 2, a.ldw_bytes = ldd * 2, a.group_bytes = down_group * 2, a.k_bytes = K * 2, a.ldy = 4 * padded_rank(rank);
   a.entries = static_cast<int>(g.entries), a.groups = g.groups, a.N = static_cast<int>(rank), a.x_rows = static_cast<int>(g.entries), a.out_kind = kOutBF16;
   // All of a rank up to 64 in one block, so that x is read once. 4099 rows of 4096: rank 16 9.0 us (8 waves 10.5; 500 rows 6.0 against
   // 5.4), rank 64 16.1 us (32 ranks per block 19.2); 7993 rows, rank 32, 18.5 us (16 rows per block 19.6,
@@ -378,7 +381,7 @@ static int expand(const Grouping& g, const void* planes, const void* up, int64_t
 
 // The chunks' sums of a gradient of so many columns.
 static size_t reduce_bytes(int64_t entries, int groups, int64_t rank, int chunk, int64_t width) {
-  return static_cast<size_t>(most_chunks(entries, groups, chunk)) * static_cast<size_t>(2 * padded_rank(rank)) * static_cast<size_t>(width) * 4;
+  return static_cast<size_t>(most_chunks(entries, groups, chunk)) * static_cast<size_t>(padded_rank(rank)) * static_cast<size_t>(width) * 4;
 }
 
 // out[a][e][n] (transposed: out[a][n][e]) = sum over a's places of planes[p][e] q[order[p]][n]; rows of q readable to a whole number of pieces.
@@ -401,9 +404,9 @@ static int reduce(const Grouping& g, int64_t rank, int chunk, const Reduction* a
     const Reduction& r = all[i];
     TileArgs& t = tiles[i];
     t.a = static_cast<const uint8_t*>(r.planes), t.b = static_cast<const uint8_t*>(r.q), t.y = r.parts, t.row_of = g.order, t.offsets = g.offsets;
-    t.lda_bytes = padded * int64_t{4}, t.ldb_bytes = r.ldq * 2, t.ldy = r.width, t.group_y = 2 * padded * r.width;
+    t.lda_bytes = padded * int64_t{8}, t.ldb_bytes = r.ldq * 2, t.ldy = r.width, t.group_y = padded * r.width;
     t.entries = static_cast<int>(g.entries), t.groups = g.groups, t.x_rows = static_cast<int>(g.entries), t.out_kind = kOutF32;
-    t.rows = 2 * padded, t.columns = static_cast<int>(r.width), t.chunk = chunk;
+    t.rows = 4 * padded, t.columns = static_cast<int>(r.width), t.chunk = chunk;
     sums[i] = {static_cast<const float*>(r.parts), static_cast<uint16_t*>(r.out), static_cast<int>(r.width), r.transposed ? 1 : 0};
     blocks[i] = most_chunks(g.entries, g.groups, chunk) * ((t.rows + kTile - 1) / kTile) * ((r.width + kTile - 1) / kTile);
     finish[i] = static_cast<int64_t>(g.groups) * (padded / 16) * ((r.width + 63) / 64);

@@ -15,10 +15,10 @@ from .linear import CompressedLinear
 
 
 def _update(y, x, down, up, scale, groups: RowGroups):
-    """The updated rows; the narrow rows between the two products (two bf16 parts of the rank rounded up to 16 each); x, down and
-    up as the kernels read them."""
+    """The updated rows; the narrow rows between the two products (three bf16 parts and zeros, of the rank rounded up to 16 each);
+    x, down and up as the kernels read them."""
     rank, outer = up.shape[2], up.shape[1]
-    planes = torch.empty(groups.entries, 2 * (-(-rank // 16) * 16), dtype=torch.bfloat16, device=x.device)
+    planes = torch.empty(groups.entries, 4 * (-(-rank // 16) * 16), dtype=torch.bfloat16, device=x.device)
     out = torch.empty(groups.entries, outer, dtype=torch.bfloat16, device=x.device)
     rows, narrow, wide, base = matrix(x, 8), matrix(down, 8), rows_of(up), rows_of(y)
     _hip.launch("ep_hip_low_rank_update", x.device,
@@ -71,8 +71,7 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         groups: the plan of `group_rows(ids, adapters)` with one id per token.
         scale: f32 [adapters] or None for ones; it gets no gradient.
 
-    Sums are f32; the narrow rows between the two products are kept in 16 bits of significand; the result is rounded to
-    bf16 once. An infinity or NaN in a row's adapter makes that row's results NaN where it reaches them. Differentiable in y, x, down and up.
+    Sums and the narrow rows between the two products are f32; the result is rounded to bf16 once. An infinity or NaN in a row's adapter makes that row's results NaN where it reaches them. Differentiable in y, x, down and up.
     """
     if not isinstance(groups, RowGroups):
         raise TypeError(f"low_rank_update takes the plan that group_rows returns, got {type(groups).__name__}")

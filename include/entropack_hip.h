@@ -467,8 +467,8 @@ int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int3
  * of none (bf16; scale NULL: ones; y NULL: zero). x: [entries][K] and down: [groups][rank][K] are read in whole 16-byte pieces:
  * 16-byte aligned, rows a multiple of 8 elements apart, zero from K to the next multiple of 8. up: [groups][N][rank].
  * planes_dev (ep_hip_low_rank_planes_bytes bytes, 16-byte aligned) receives the narrow rows scale[g] x[order[p]] down[g]^T in grouped
- * order, as two bf16 parts per value: columns [0, padded) the rounded value, [padded, 2 padded) the rounded remainder, padded =
- * rank rounded up to 16. The gradient of up reads them.
+ * order, as three bf16 parts that add up to the f32 value: for every 16 ranks 64 columns, 16 rounded values, 16 rounded remainders, 16 of
+ * what then remains, 16 zeros. The gradient of up reads them.
  * _grad: any of grad_x [entries][K] (rows of no adapter zero), grad_down [groups][rank][K] and grad_up [groups][N][rank] (contiguous),
  * each absent when NULL, from grad_dev, the output's gradient [entries][N], read in whole pieces as x is; up is needed for the
  * first two, down for the first, x for the second, planes (of the forward) for the third. workspace: 256-byte aligned. */

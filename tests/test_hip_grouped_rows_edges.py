@@ -1,0 +1,77 @@
+"""GPU tests of the operators on grouped rows where results are small against what they are sums of, where operands lie oddly, at
+sizes that other kernels serve, and through the entry points of the C library. Against plain implementations in 64 bits.
+
+Tolerances: products of two bf16 numbers are exact in f32; every addition of a sum, in any order and whichever way the matrix cores
+round, is off by at most a whole unit in the last place, 2^-23 of the sum of the magnitudes; a rounding to bf16 by half a step, 2^-8 of
+the value.
+"""
+import pytest
+import torch
+
+import entropack_amd as ep
+
+pytestmark = pytest.mark.gpu
+HALF_BF16, STEP_F32 = 2.0 ** -8, 2.0 ** -23
+
+
+def _within(got, expect, bound):
+    off = (got.double() - expect).abs()
+    assert torch.isfinite(got.double()).all()
+    worst = (off - bound).max().item() if off.numel() else -1.0
+    assert worst <= 0.0, f"off by {worst} more than the bound; largest difference {off.max().item()}"
+
+
+@pytest.mark.parametrize("tokens", [20, 40], ids=["few rows", "many rows"])       # 16 rows per block in the product with `up`, and 64
+def test_narrow_rows_of_an_adapter_lose_nothing(tokens):
+    """One feature, rank one: h = s (x d) is one product of three numbers, exact but for the rounding of an f32. y is the update's negative
+    rounded to bf16, so that what is left is some 2^-9 of the update and shows what of it was lost on the way. Three parts' products
+    and y make four additions; with the rounding of h eight steps bound them, of |y| + |update|."""
+    outer = 4096
+    source = torch.Generator(device="cuda").manual_seed(7)
+    make = lambda *shape: torch.randn(*shape, device="cuda", generator=source).bfloat16()
+    plan = ep.group_rows(torch.zeros(tokens, dtype=torch.int64, device="cuda"), 1)
+    x, down, up, scale = make(tokens, 1), make(1, 1, 1), make(1, outer, 1), 0.5 + torch.rand(1, device="cuda", generator=source)
+    update = (scale.double() * x.double() * down[0, 0, 0].double()) * up[0, :, 0].double()
+    y = (-update).bfloat16()
+    out = ep.low_rank_update(y, x, down, up, plan, scale)
+    want = y.double() + update
+    _within(out, want, HALF_BF16 * want.abs() + 8 * STEP_F32 * (y.double().abs() + update.abs()))
+
+
+def test_narrow_rows_of_an_adapters_gradients_lose_nothing():
+    """The same for the gradients: each is a sum of two terms that cancel to some 2^-9 of either. Of x: two ranks, whose second row of
+    `down` is chosen so; of `down` and `up`: two tokens, the second's row of the other operand chosen so."""
+    wide = 4096
+    source = torch.Generator(device="cuda").manual_seed(8)
+    make = lambda *shape: torch.randn(*shape, device="cuda", generator=source).bfloat16()
+    scale = 0.5 + torch.rand(1, device="cuda", generator=source)
+    s = scale.double()
+
+    def gradients(x, down, up, dout):
+        plan = ep.group_rows(torch.zeros(len(x), dtype=torch.int64, device="cuda"), 1)
+        leaves = [t.requires_grad_(True) for t in (x, down, up)]
+        return torch.autograd.grad(ep.low_rank_update(torch.zeros_like(dout), *leaves, plan, scale), leaves, dout)
+
+    def check(got, first, second):                           # two terms of three parts each: eight additions and two roundings of an f32
+        want = first + second
+        assert want.abs().median() < 2.0 ** -8 * first.abs().median()
+        _within(got, want, HALF_BF16 * want.abs() + 10 * STEP_F32 * (first.abs() + second.abs()))
+
+    # gradient of x: e_0 down[0] + e_1 down[1] with e_r = s dout up[r]
+    dout, up, x = make(1, 1), make(1, 1, 2), make(1, wide)
+    e = s * dout.double()[0, 0] * up.double()[0, 0]
+    down = make(1, 2, wide)
+    down[0, 1] = (-e[0] * down[0, 0].double() / e[1]).bfloat16()
+    check(gradients(x, down, up, dout)[0][0], e[0] * down[0, 0].double(), e[1] * down[0, 1].double())
+
+    # gradient of down: e_0 x[0] + e_1 x[1] with e_t = s dout[t] up
+    dout, up, x, down = make(2, 1), make(1, 1, 1), make(2, wide), make(1, 1, wide)
+    e = s * dout.double()[:, 0] * up.double()[0, 0, 0]
+    x[1] = (-e[0] * x[0].double() / e[1]).bfloat16()
+    check(gradients(x, down, up, dout)[1][0, 0], e[0] * x[0].double(), e[1] * x[1].double())
+
+    # gradient of up: h_0 dout[0] + h_1 dout[1] with h_t = s x[t] down
+    dout, up, x, down = make(2, wide), make(1, wide, 1), make(2, 1), make(1, 1, 1)
+    h = s * x.double()[:, 0] * down.double()[0, 0, 0]
+    dout[1] = (-h[0] * dout[0].double() / h[1]).bfloat16()
+    check(gradients(x, down, up, dout)[2][0, :, 0], h[0] * dout[0].double(), h[1] * dout[1].double())
