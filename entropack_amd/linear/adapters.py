@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from ..backends import hip as _hip
-from .groups import RowGroups, device_of, first_order, matrix, rows_of
+from .groups import RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of
 from .linear import CompressedLinear
 
 
@@ -71,7 +71,8 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         groups: the plan of `group_rows(ids, adapters)` with one id per token.
         scale: f32 [adapters] or None for ones; it gets no gradient.
 
-    Sums and the narrow rows between the two products are f32; the result is rounded to bf16 once. An infinity or NaN in a row's adapter makes that row's results NaN where it reaches them. Differentiable in y, x, down and up.
+    Sums and the narrow rows between the two products are f32; the result is rounded to bf16 once. An infinity or NaN in a row's adapter makes that row's results NaN where it reaches them. Differentiable in y, x, down and
+    up, in reverse mode.
     """
     if not isinstance(groups, RowGroups):
         raise TypeError(f"low_rank_update takes the plan that group_rows returns, got {type(groups).__name__}")
@@ -90,6 +91,7 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         raise ValueError("low_rank_update needs at least one feature and rank one")
     if down.shape[1] > 4096:
         raise ValueError(f"low_rank_update takes ranks up to 4096, got {down.shape[1]}")
+    refuse_tangents("low_rank_update", y, x, down, up, scale)
     if scale is not None:
         if tuple(scale.shape) != (groups.groups,):
             raise ValueError(f"low_rank_update takes one scale per adapter, got shape {tuple(scale.shape)}")

@@ -17,7 +17,7 @@ import torch
 from ..backends import hip as _hip
 from ..compression import BatchDecompressor
 from . import kernels
-from .groups import RowGroups, device_of, first_order, matrix, rows_of, sum_entries
+from .groups import RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of, sum_entries
 from .linear import CompressedINT8Linear, CompressedLinear
 
 
@@ -125,7 +125,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
         groups: the plan of `group_rows`.
         bias: bf16 [groups, out_features] or None.
 
-    Sums are f32, rounded to bf16 once. Differentiable in x, weight and bias. Feature counts that are no multiple of 8 are
+    Sums are f32, rounded to bf16 once. Differentiable in x, weight and bias, in reverse mode. Feature counts that are no multiple of 8 are
     padded, which copies the operand.
     """
     _check_groups("grouped_linear", x, weight, groups, bias, x_grouped)
@@ -133,6 +133,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
         if tensor is not None and tensor.dtype != torch.bfloat16:
             raise TypeError(f"grouped_linear takes bfloat16 operands, got {name} in {tensor.dtype}")
     device_of("grouped_linear", x, weight, groups.order, bias)
+    refuse_tangents("grouped_linear", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GroupedLinear.apply(x, weight, bias, groups, x_grouped)
     return _forward(x, weight, bias, groups, x_grouped)
@@ -157,6 +158,7 @@ def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups
         raise ValueError(f"grouped_int8_linear takes {x.shape[0]} activation scales and weight scales of shape {tuple(weight.shape[:2])}, "
                          f"got {tuple(x_scale.shape)} and {tuple(weight_scale.shape)}")
     device = device_of("grouped_int8_linear", x, weight, groups.order, x_scale, weight_scale, bias)
+    refuse_tangents("grouped_int8_linear", x_scale, weight_scale, bias)
     outer = weight.shape[1]
     y = torch.empty(groups.entries, outer, dtype=out_dtype, device=device)
     if y.numel() == 0:
@@ -274,6 +276,7 @@ class CompressedGroupedLinear(torch.nn.Module):
         if x.dtype != torch.bfloat16:
             raise TypeError(f"CompressedGroupedLinear runs in bfloat16, got {x.dtype}")
         device_of("CompressedGroupedLinear", x)
+        refuse_tangents("CompressedGroupedLinear", x)
         if not isinstance(groups, RowGroups):
             raise TypeError(f"CompressedGroupedLinear takes the plan that group_rows returns, got {type(groups).__name__}")
         if groups.groups != self.groups:

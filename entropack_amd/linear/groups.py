@@ -15,6 +15,7 @@ import dataclasses
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from ..backends import hip as _hip
 
@@ -37,6 +38,15 @@ def device_of(name: str, *tensors: torch.Tensor | None) -> torch.device:
         elif tensor.device != device:
             raise ValueError(f"{name}: all operands must be on one device, got {device} and {tensor.device}")
     return device
+
+
+def refuse_tangents(name: str, *tensors: torch.Tensor | None) -> None:
+    """The operators have gradients, no Jacobian-vector products. A tensor with a tangent need not ask for a gradient, so a call on it could
+    return a result whose tangent is missing: such a call raises. (The level is asked for first: outside of one no tensor has a tangent.)"""
+    if forward_ad._current_level < 0:
+        return
+    if any(tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None for tensor in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative (jvp); detach the operand or take the gradient in reverse mode")
 
 
 def matrix(tensor: torch.Tensor, pieces: int) -> torch.Tensor:
@@ -75,6 +85,7 @@ def first_order(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        refuse_tangents("the gradient of an operator on grouped rows", *grads)
         return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 
@@ -208,7 +219,7 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weight: torch.Tensor | None
         weight: f32 or bf16, the shape of the ids, or None for ones (the router's weights).
 
     Entries of no group add nothing, whatever y and weight hold there. Sums are f32, rounded to bf16 once. Differentiable
-    in y and weight.
+    in y and weight, in reverse mode.
     """
     if not isinstance(groups, RowGroups):
         raise TypeError(f"combine_rows takes the plan that group_rows returns, got {type(groups).__name__}")
@@ -222,6 +233,7 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weight: torch.Tensor | None
         if tuple(weight.shape) not in ({(groups.tokens, groups.per_row)} | ({(groups.tokens,)} if groups.per_row == 1 else set())):
             raise ValueError(f"combine_rows takes weights of shape {(groups.tokens, groups.per_row)}, got {tuple(weight.shape)}")
     device_of("combine_rows", y, groups.order, weight)
+    refuse_tangents("combine_rows", y, weight)
     if torch.is_grad_enabled() and (y.requires_grad or (weight is not None and weight.requires_grad)):
         return _CombineRows.apply(y, weight, groups)
     return _combine(y, weight, groups)[0]

@@ -1,0 +1,74 @@
+"""The operators on grouped rows without a device, continued: derivatives that they do not give, layers moved, cast and put together in
+ways they cannot serve, sizes beyond a launch. Kernels are replaced by nothing where a call would reach them: what is tested is what
+the call refuses, or what it hands on."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import entropack_amd as ep
+from entropack_amd.backends import hip
+from entropack_amd.linear import adapters, grouped, groups
+
+
+def _plan(tokens=3, per_row=2, count=4):
+    entries = tokens * per_row
+    index = torch.arange(entries, dtype=torch.int32)
+    return ep.RowGroups(index, torch.full((count + 1,), entries, dtype=torch.int32), index.clone(), index // per_row, count, tokens, per_row)
+
+
+def _bf16(*shape):
+    return torch.ones(*shape, dtype=torch.bfloat16)
+
+
+@pytest.fixture
+def no_device(monkeypatch):
+    """The operators on host tensors, every kernel replaced by nothing; yields the names of those that were called."""
+    called = []
+    monkeypatch.setattr(hip, "launch", lambda name, *rest: called.append(name))
+    for module in (adapters, grouped, groups):
+        monkeypatch.setattr(module, "device_of", lambda name, *tensors: torch.device("cpu"))
+    return called
+
+
+OPERATORS = [("grouped_linear", lambda x, w, b: ep.grouped_linear(x, w, _plan(), b), (_bf16(3, 8), _bf16(4, 5, 8), _bf16(4, 5))),
+             ("combine_rows", lambda y, w: ep.combine_rows(y, _plan(), w), (_bf16(6, 8), torch.ones(3, 2))),
+             ("low_rank_update", lambda y, x, d, u: ep.low_rank_update(y, x, d, u, _plan(per_row=1)), (_bf16(3, 10), _bf16(3, 8), _bf16(4, 2, 8), _bf16(4, 10, 2))),
+             ("low_rank_update's scale", lambda s: ep.low_rank_update(_bf16(3, 10), _bf16(3, 8), _bf16(4, 2, 8), _bf16(4, 10, 2), _plan(per_row=1), s), (torch.ones(4),)),
+             ("grouped_int8_linear", lambda sx, sw, b: ep.grouped_int8_linear(torch.ones(3, 16, dtype=torch.int8), torch.ones(4, 5, 16, dtype=torch.int8), _plan(), sx, sw, b),
+              (torch.ones(3), torch.ones(4, 5), _bf16(4, 5)))]
+
+
+@pytest.mark.parametrize("name,run,operands", OPERATORS, ids=[o[0] for o in OPERATORS])
+@pytest.mark.parametrize("recording", [True, False], ids=["grad", "no_grad"])
+def test_forward_mode_derivatives_are_refused_not_dropped(no_device, name, run, operands, recording):
+    run(*operands)                                                                       # without tangents the call is fine
+    for which in range(len(operands)):
+        def of_one(t):
+            return run(*[t if i == which else o for i, o in enumerate(operands)])
+
+        with torch.set_grad_enabled(recording):
+            before = len(no_device)
+            with forward_ad.dual_level():
+                assert forward_ad.unpack_dual(run(*operands)).tangent is None                # nor does a level without tangents matter
+                with pytest.raises((RuntimeError, ValueError), match="forward-mode|jvp|JVP"):
+                    of_one(forward_ad.make_dual(operands[which], torch.ones_like(operands[which])))
+            with pytest.raises((RuntimeError, ValueError)):
+                torch.func.jvp(of_one, (operands[which],), (torch.ones_like(operands[which]),))
+            with pytest.raises((RuntimeError, ValueError)):
+                torch.func.vmap(of_one)(operands[which].unsqueeze(0).expand(2, *operands[which].shape).clone())
+
+
+def test_a_mixtures_forward_mode_derivative_is_refused(no_device):
+    experts = ep.CompressedGroupedLinear([ep.CompressedLinear(8, 5) for _ in range(4)])
+    experts._stacked = lambda device: _bf16(4, 5, 8)
+    assert experts(_bf16(3, 8), _plan()).shape == (6, 5)
+    with forward_ad.dual_level(), pytest.raises((RuntimeError, ValueError), match="forward-mode|jvp|JVP"):
+        experts(forward_ad.make_dual(_bf16(3, 8), _bf16(3, 8)), _plan())
+
+
+@pytest.mark.parametrize("name,run,operands", OPERATORS[:3], ids=[o[0] for o in OPERATORS[:3]])
+def test_a_gradient_with_a_tangent_is_refused(no_device, name, run, operands):
+    leaves = [t.clone().requires_grad_(True) for t in operands]
+    out = run(*leaves)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        torch.autograd.grad(out, leaves[0], forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
