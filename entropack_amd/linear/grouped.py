@@ -175,18 +175,20 @@ def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups
 
 
 class _CompressedGrouped(torch.autograd.Function):
-    """The forward on decoded weights with the gradient of the activations; the weights are decoded again for it (they are
-    frozen and get no gradient), as in the layers' own fused forward."""
+    """The forward on decoded weights with the gradients of the activations and of the biases; the weights are decoded again for the
+    first (they are frozen and get no gradient), as in the layers' own fused forward."""
 
     @staticmethod
-    def forward(ctx, x, layer, groups, x_grouped):
+    def forward(ctx, x, biases, layer, groups, x_grouped):
         ctx.layer, ctx.groups, ctx.x_grouped = layer, groups, x_grouped
-        return layer._product(x.detach(), groups, x_grouped)
+        return layer._product(x.detach(), biases, groups, x_grouped)
 
     @staticmethod
     @first_order
     def backward(ctx, grad):
-        return _grad_rows(grad, ctx.layer.dequantize(grad.device).to(grad.dtype), ctx.groups, ctx.x_grouped), None, None, None
+        need_x, need_biases = ctx.needs_input_grad[:2]
+        return (_grad_rows(grad, ctx.layer.dequantize(grad.device).to(grad.dtype), ctx.groups, ctx.x_grouped) if need_x else None,
+                _grad_bias(grad, ctx.groups) if need_biases else None, None, None, None)
 
 
 class CompressedGroupedLinear(torch.nn.Module):
@@ -195,7 +197,8 @@ class CompressedGroupedLinear(torch.nn.Module):
     `experts`: `CompressedLinear` layers (bf16 containers) or `CompressedINT8Linear` layers, one class, one shape, with
     biases in all of them or in none. They stay ordinary submodules: `state_dict` holds `experts.<i>.weight.entropack_quant_state`
     and so on. A forward decodes all experts (in one pass when their weights are `lattice_rans` containers), then runs
-    `grouped_linear` or, for int8 experts, the row quantiser and `grouped_int8_linear`. Differentiable in x. The first forward
+    `grouped_linear` or, for int8 experts, the row quantiser and `grouped_int8_linear`. Differentiable in x and in the biases (which the
+    layers keep frozen unless asked otherwise). The first forward
     plans the decode, which copies to the device: run one before capturing a graph.
     """
 
@@ -254,9 +257,8 @@ class CompressedGroupedLinear(torch.nn.Module):
         apart = row * self.out_features if len(views) == 1 else (views[1].data_ptr() - views[0].data_ptr()) // size    # one shape, so even steps
         return torch.as_strided(views[0], (len(views), self.out_features, self.in_features), (apart, row, 1))
 
-    def _product(self, x: torch.Tensor, groups: RowGroups, x_grouped: bool) -> torch.Tensor:
+    def _product(self, x: torch.Tensor, biases: torch.Tensor | None, groups: RowGroups, x_grouped: bool) -> torch.Tensor:
         weight = self._stacked(x.device)
-        biases = None if self.experts[0].bias is None else torch.stack([expert._bias_on(x.device) for expert in self.experts])
         if not self._int8:
             return grouped_linear(x, weight, groups, biases, x_grouped=x_grouped)
         first = self.experts[0]
@@ -286,9 +288,10 @@ class CompressedGroupedLinear(torch.nn.Module):
             raise ValueError(f"CompressedGroupedLinear takes x of shape {(rows, self.in_features)}, got {tuple(x.shape)}")
         if groups.entries == 0:
             return x.new_zeros(0, self.out_features) + x.sum() * 0
-        if torch.is_grad_enabled() and x.requires_grad:
-            return _CompressedGrouped.apply(x, self, groups, x_grouped)
-        return self._product(x, groups, x_grouped)
+        biases = None if self.experts[0].bias is None else torch.stack([expert._bias_on(x.device) for expert in self.experts])
+        if torch.is_grad_enabled() and (x.requires_grad or (biases is not None and biases.requires_grad)):
+            return _CompressedGrouped.apply(x, biases, self, groups, x_grouped)
+        return self._product(x, biases, groups, x_grouped)
 
     def extra_repr(self) -> str:
         return f"experts={self.groups}, in_features={self.in_features}, out_features={self.out_features}"

@@ -72,3 +72,16 @@ def test_a_gradient_with_a_tangent_is_refused(no_device, name, run, operands):
     out = run(*leaves)
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         torch.autograd.grad(out, leaves[0], forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+@pytest.mark.parametrize("of_x", [False, True], ids=["biases alone", "and x"])
+def test_a_mixture_hands_its_biases_their_gradients(no_device, monkeypatch, of_x):
+    monkeypatch.setattr(grouped, "_grad_rows", lambda grad, weight, plan, x_grouped: torch.full((3, 8), 2.0, dtype=grad.dtype))
+    monkeypatch.setattr(grouped, "_grad_bias", lambda grad, plan: torch.arange(20.0, dtype=grad.dtype).reshape(4, 5))
+    layer = ep.CompressedGroupedLinear([ep.CompressedLinear(8, 5) for _ in range(4)])
+    layer._stacked = lambda device: _bf16(4, 5, 8)
+    biases = [expert.bias.requires_grad_(True) for expert in layer.experts]
+    x = _bf16(3, 8).requires_grad_(of_x)
+    layer(x, _plan()).sum().backward()
+    assert torch.equal(torch.stack([bias.grad for bias in biases]), torch.arange(20.0).reshape(4, 5).bfloat16())
+    assert (x.grad is not None) == of_x

@@ -75,3 +75,35 @@ def test_narrow_rows_of_an_adapters_gradients_lose_nothing():
     h = s * x.double()[:, 0] * down.double()[0, 0, 0]
     dout[1] = (-h[0] * dout[0].double() / h[1]).bfloat16()
     check(gradients(x, down, up, dout)[2][0, :, 0], h[0] * dout[0].double(), h[1] * dout[1].double())
+
+
+def _linears(experts, outer, inner, bias=True):
+    torch.manual_seed(4)
+    return [torch.nn.Linear(inner, outer, bias=bias, dtype=torch.bfloat16) for _ in range(experts)]
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("of_x", [False, True], ids=["biases alone", "and x"])
+def test_biases_of_compressed_experts_that_train_get_their_gradient(int8, of_x):
+    experts, outer, inner, tokens = 3, 72, 128, 40
+    options = {"int8": True} if int8 else {"config": ep.EntroPackLossyConfig(target_bpp=4.0)}
+    layer = ep.CompressedGroupedLinear.from_linears(_linears(experts, outer, inner), **options).cuda()
+    ids = torch.randint(-1, experts, (tokens, 2), generator=torch.Generator().manual_seed(1)).cuda()
+    plan = ep.group_rows(ids, experts)
+    x = torch.randn(tokens, inner, device="cuda").bfloat16()
+    frozen = layer(x, plan)
+    biases = [expert.bias.requires_grad_(True) for expert in layer.experts]
+    leaves = biases + ([x.requires_grad_(True)] if of_x else [])
+    y = layer(x, plan)
+    assert torch.equal(y, frozen)
+    dy = torch.randn(y.shape, device="cuda").bfloat16()
+    grads = torch.autograd.grad(y, leaves, dy)
+    for g in range(experts):
+        rows = dy[int(plan.offsets[g]):int(plan.offsets[g + 1])].double()
+        _within(grads[g], rows.sum(0), HALF_BF16 * rows.sum(0).abs() + len(rows) * STEP_F32 * rows.abs().sum(0) * 1.01)
+    if of_x:
+        plain = x.detach().requires_grad_(True)
+        want = torch.autograd.grad(ep.grouped_linear(plain, layer.dequantize().bfloat16(), plan), plain, dy)[0]
+        assert torch.equal(grads[experts], want)
+    with torch.no_grad():
+        assert torch.equal(layer(x, plan), frozen)
