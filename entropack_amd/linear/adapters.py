@@ -114,7 +114,8 @@ class AdaptedLinear(torch.nn.Module):
         adapters: how many the bank holds. rank: of every adapter; a smaller one is stored padded with zeros.
 
     `down` starts with small random values and `up` with zeros, so that a new adapter changes nothing until it is trained or set;
-    both are trainable parameters. `scale` is a buffer of ones.
+    both are trainable parameters. `scale` is a buffer of ones. Casting the layer (`.to(dtype)`, `.half()`, ..) casts none of the three: the
+    kernels take the adapters in bf16 and the scales in f32.
     """
 
     def __init__(self, base: CompressedLinear, adapters: int, rank: int):
@@ -137,6 +138,15 @@ class AdaptedLinear(torch.nn.Module):
     @property
     def rank(self) -> int:
         return self.down.shape[1]
+
+    def _apply(self, fn, recurse=True):
+        def keep(tensor):
+            moved = fn(tensor)
+            return moved if moved.dtype == tensor.dtype else tensor.to(device=moved.device)
+
+        if recurse:
+            self.base._apply(fn)
+        return super()._apply(keep, recurse=False)
 
     @torch.no_grad()
     def set_adapter(self, index: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:

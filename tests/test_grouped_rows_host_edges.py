@@ -85,3 +85,19 @@ def test_a_mixture_hands_its_biases_their_gradients(no_device, monkeypatch, of_x
     layer(x, _plan()).sum().backward()
     assert torch.equal(torch.stack([bias.grad for bias in biases]), torch.arange(20.0).reshape(4, 5).bfloat16())
     assert (x.grad is not None) == of_x
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: torch.nn.Sequential(m).half()[0]], ids=["bf16", "half", "double", "inside a model"])
+def test_casting_an_adapted_layer_leaves_its_bank_as_the_kernels_take_it(cast):
+    layer = ep.AdaptedLinear(ep.CompressedLinear(16, 8), 3, 4)
+    layer.set_adapter(1, torch.randn(4, 16), torch.randn(8, 4), scale=1.0 / 3.0)
+    down, up, scale = layer.down.detach().clone(), layer.up.detach().clone(), layer.scale.clone()
+    parameters = list(layer.parameters())
+    cast(layer)
+    assert layer.down.dtype == layer.up.dtype == torch.bfloat16 and layer.scale.dtype == torch.float32
+    assert torch.equal(layer.down, down) and torch.equal(layer.up, up) and torch.equal(layer.scale, scale) and layer.down.requires_grad
+    assert all(a is b for a, b in zip(parameters, layer.parameters()))              # an optimiser's own
+    meta = layer.to("meta")
+    assert meta.down.device.type == meta.scale.device.type == "meta" and meta.scale.dtype == torch.float32
+    empty = meta.to_empty(device="cpu")
+    assert empty.up.device.type == "cpu" and empty.up.dtype == torch.bfloat16
