@@ -157,10 +157,11 @@ class AdaptedLinear(torch.nn.Module):
         if rank > self.rank or tuple(down.shape) != (rank, self.base.in_features) or tuple(up.shape) != (self.base.out_features, rank):
             raise ValueError(f"an adapter of this bank has down [r, {self.base.in_features}] and up [{self.base.out_features}, r] with r up to "
                              f"{self.rank}, got {tuple(down.shape)} and {tuple(up.shape)}")
-        self.down[index].zero_()
-        self.up[index].zero_()
-        self.down[index, :rank].copy_(down)
-        self.up[index, :, :rank].copy_(up)
+        fresh_down, fresh_up = torch.zeros_like(self.down[index]), torch.zeros_like(self.up[index])    # the source may be a part of this slot
+        fresh_down[:rank].copy_(down)
+        fresh_up[:, :rank].copy_(up)
+        self.down[index].copy_(fresh_down)
+        self.up[index].copy_(fresh_up)
         self.scale[index] = scale
 
     def forward(self, x: torch.Tensor, groups: RowGroups) -> torch.Tensor:

@@ -101,3 +101,12 @@ def test_casting_an_adapted_layer_leaves_its_bank_as_the_kernels_take_it(cast):
     assert meta.down.device.type == meta.scale.device.type == "meta" and meta.scale.dtype == torch.float32
     empty = meta.to_empty(device="cpu")
     assert empty.up.device.type == "cpu" and empty.up.dtype == torch.bfloat16
+
+
+def test_an_adapter_set_from_a_part_of_its_own_slot():
+    layer = ep.AdaptedLinear(ep.CompressedLinear(16, 8), 2, 4)
+    layer.set_adapter(1, torch.randn(4, 16), torch.randn(8, 4))
+    down, up = layer.down[1].detach().clone(), layer.up[1].detach().clone()
+    layer.set_adapter(1, layer.down[1, 1:3], layer.up[1, :, 1:3], scale=2.0)         # two of its four ranks kept
+    assert torch.equal(layer.down[1, :2], down[1:3]) and torch.equal(layer.up[1, :, :2], up[:, 1:3])
+    assert layer.down[1, 2:].eq(0).all() and layer.up[1, :, 2:].eq(0).all() and layer.scale.tolist() == [1.0, 2.0]
