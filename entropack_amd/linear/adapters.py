@@ -10,8 +10,11 @@ from __future__ import annotations
 import torch
 
 from ..backends import hip as _hip
-from .groups import RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of
+from .groups import MAX_GROUPS, RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of
 from .linear import CompressedLinear
+
+
+MAX_RANK = 4096
 
 
 def _update(y, x, down, up, scale, groups: RowGroups):
@@ -89,8 +92,8 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
                          f"got {tuple(x.shape)} and {tuple(y.shape)}")
     if 0 in down.shape or 0 in up.shape:
         raise ValueError("low_rank_update needs at least one feature and rank one")
-    if down.shape[1] > 4096:
-        raise ValueError(f"low_rank_update takes ranks up to 4096, got {down.shape[1]}")
+    if down.shape[1] > MAX_RANK:
+        raise ValueError(f"low_rank_update takes ranks up to {MAX_RANK}, got {down.shape[1]}")
     refuse_tangents("low_rank_update", y, x, down, up, scale)
     if scale is not None:
         if tuple(scale.shape) != (groups.groups,):
@@ -122,9 +125,9 @@ class AdaptedLinear(torch.nn.Module):
         super().__init__()
         if not isinstance(base, CompressedLinear):
             raise TypeError(f"AdaptedLinear takes a compressed linear layer, got {type(base).__name__}")
-        for name, value in (("adapters", adapters), ("rank", rank)):
-            if isinstance(value, bool) or not isinstance(value, int) or value < 1:
-                raise ValueError(f"{name} must be a positive integer, got {value!r}")
+        for name, value, most in (("adapters", adapters, MAX_GROUPS), ("rank", rank, MAX_RANK)):
+            if isinstance(value, bool) or not isinstance(value, int) or not 1 <= value <= most:
+                raise ValueError(f"{name} must be an integer from 1 to {most}, got {value!r}")
         self.base = base
         device = base.device
         self.down = torch.nn.Parameter(torch.randn(adapters, rank, base.in_features, device=device).mul_(base.in_features ** -0.5).bfloat16())

@@ -17,7 +17,7 @@ import torch
 from ..backends import hip as _hip
 from ..compression import BatchDecompressor
 from . import kernels
-from .groups import RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of, sum_entries
+from .groups import MAX_GROUPS, RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of, sum_entries
 from .linear import CompressedINT8Linear, CompressedLinear
 
 
@@ -207,6 +207,8 @@ class CompressedGroupedLinear(torch.nn.Module):
         experts = list(experts)
         if not experts:
             raise ValueError("CompressedGroupedLinear needs at least one expert")
+        if len(experts) > MAX_GROUPS:
+            raise ValueError(f"CompressedGroupedLinear takes at most {MAX_GROUPS} experts, got {len(experts)}")
         first = experts[0]
         kind = CompressedINT8Linear if isinstance(first, CompressedINT8Linear) else CompressedLinear
         for expert in experts:

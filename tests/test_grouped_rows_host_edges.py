@@ -110,3 +110,15 @@ def test_an_adapter_set_from_a_part_of_its_own_slot():
     layer.set_adapter(1, layer.down[1, 1:3], layer.up[1, :, 1:3], scale=2.0)         # two of its four ranks kept
     assert torch.equal(layer.down[1, :2], down[1:3]) and torch.equal(layer.up[1, :, :2], up[:, 1:3])
     assert layer.down[1, 2:].eq(0).all() and layer.up[1, :, 2:].eq(0).all() and layer.scale.tolist() == [1.0, 2.0]
+
+
+def test_a_bank_that_no_forward_could_use_is_refused():
+    base = ep.CompressedLinear(16, 8)
+    for count, rank in ((groups.MAX_GROUPS + 1, 1), (1, 4097)):
+        with pytest.raises(ValueError, match="from 1 to"):
+            ep.AdaptedLinear(base, count, rank)
+    assert ep.AdaptedLinear(base, groups.MAX_GROUPS, 1).adapters == 896 and ep.AdaptedLinear(base, 1, 4096).rank == 4096
+    experts = [ep.CompressedLinear(16, 8) for _ in range(groups.MAX_GROUPS + 1)]
+    with pytest.raises(ValueError, match="at most 896"):
+        ep.CompressedGroupedLinear(experts)
+    assert ep.CompressedGroupedLinear(experts[:-1]).groups == 896
