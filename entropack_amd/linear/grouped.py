@@ -199,7 +199,8 @@ class CompressedGroupedLinear(torch.nn.Module):
     and so on. A forward decodes all experts (in one pass when their weights are `lattice_rans` containers), then runs
     `grouped_linear` or, for int8 experts, the row quantiser and `grouped_int8_linear`. Differentiable in x and in the biases (which the
     layers keep frozen unless asked otherwise). The first forward
-    plans the decode, which copies to the device: run one before capturing a graph.
+    plans the decode, which copies to the device: run one before capturing a graph. The plan is made again when a container changes or the
+    layer moves; of experts kept on the host it holds a copy of the containers on the device.
     """
 
     def __init__(self, experts):
@@ -226,7 +227,7 @@ class CompressedGroupedLinear(torch.nn.Module):
         self.experts = torch.nn.ModuleList(experts)
         self.in_features, self.out_features = first.in_features, first.out_features
         self._int8 = kind is CompressedINT8Linear
-        self._decoder = None            # (the containers' payloads it was planned for, BatchDecompressor)
+        self._decoder = None            # (device, the experts' payloads it was planned for, BatchDecompressor)
 
     @classmethod
     def from_linears(cls, linears, *, int8: bool = False, **kwargs) -> "CompressedGroupedLinear":
@@ -238,21 +239,31 @@ class CompressedGroupedLinear(torch.nn.Module):
         # A decode plan holds addresses of this object's containers: a copy makes its own.
         return {**self.__dict__, "_decoder": None}
 
+    def _apply(self, fn, recurse=True):
+        self._decoder = None            # it keeps the containers that are about to be left behind
+        return super()._apply(fn, recurse=recurse)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._decoder = None
+        super()._load_from_state_dict(*args, **kwargs)
+
     @property
     def groups(self) -> int:
         return len(self.experts)
 
     def _stacked(self, device: torch.device) -> torch.Tensor:
         """All experts' containers decoded: [experts, out_features, in_features] in the containers' dtype."""
-        containers = [expert._container().to(device=device, dtype=expert.container_dtype) for expert in self.experts]
+        containers = [expert._container() for expert in self.experts]
         if any(container.compress_method != "lattice_rans" for container in containers):
             return torch.stack([expert.codes(device) if self._int8 else expert.dequantize(device).to(expert.container_dtype) for expert in self.experts])
-        payloads = tuple(container.buffers["payload"] for container in containers)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         held = self._decoder
-        if held is None or len(held[0]) != len(payloads) or any(a is not b for a, b in zip(held[0], payloads)):
-            held = self._decoder = (payloads, BatchDecompressor(containers, self.experts[0]._decode_config))
-        arena = torch.empty(held[1].arena_bytes, dtype=torch.uint8, device=device)
-        views = held[1](arena)
+        if held is None or held[0] != device or any(container.buffers["payload"] is not payload for container, payload in zip(containers, held[1])):
+            here = [container.to(device=device, dtype=expert.container_dtype) for container, expert in zip(containers, self.experts)]
+            held = self._decoder = (device, [container.buffers["payload"] for container in containers], BatchDecompressor(here, self.experts[0]._decode_config))
+        arena = torch.empty(held[2].arena_bytes, dtype=torch.uint8, device=device)
+        views = held[2](arena)
         if any(view.untyped_storage().data_ptr() != arena.data_ptr() for view in views):
             return torch.stack(views)                        # a type the decode stores as another and converts
         size, row = views[0].element_size(), views[0].stride(0)

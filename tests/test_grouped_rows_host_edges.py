@@ -122,3 +122,39 @@ def test_a_bank_that_no_forward_could_use_is_refused():
     with pytest.raises(ValueError, match="at most 896"):
         ep.CompressedGroupedLinear(experts)
     assert ep.CompressedGroupedLinear(experts[:-1]).groups == 896
+
+
+def test_a_mixture_that_moves_or_is_loaded_lets_go_of_its_decode_plan():
+    layer = ep.CompressedGroupedLinear([ep.CompressedLinear(16, 8) for _ in range(2)])
+    for change in (lambda: layer.cpu(), lambda: layer.to(torch.bfloat16), lambda: torch.nn.Sequential(layer).cpu(),
+                   lambda: layer.load_state_dict(layer.state_dict(), strict=False), lambda: torch.nn.Sequential(layer).load_state_dict({}, strict=False)):
+        layer._decoder = object()
+        change()
+        assert layer._decoder is None
+
+
+def test_a_mixture_plans_once_wherever_its_containers_are(monkeypatch):
+    """Neither containers on another device than x nor a cast, which both need new tensors for the decode, make a plan per call."""
+    config, made = ep.EntroPackLossyConfig(target_bpp=4.0, execution_backend="eager"), []
+
+    class Plan:
+        arena_bytes = 2 * 8 * 16 * 2
+
+        def __init__(self, containers, config):
+            made.append([container.dtype for container in containers])
+
+        def __call__(self, arena):
+            return list(arena.view(torch.bfloat16).view(2, 8, 16).unbind(0))
+
+    monkeypatch.setattr(grouped, "BatchDecompressor", Plan)
+    layer = ep.CompressedGroupedLinear.from_linears([torch.nn.Linear(16, 8, dtype=torch.bfloat16) for _ in range(2)], config=config)
+    layer.float()
+    for _ in range(3):
+        assert layer._stacked(torch.device("cpu")).shape == (2, 8, 16)
+    assert made == [[torch.bfloat16] * 2]
+    layer._stacked(torch.device("meta"))                                               # another device, another plan
+    assert len(made) == 2
+    layer.experts[1].compress_weight(torch.randn(8, 16))                               # another container, another plan
+    layer._stacked(torch.device("meta"))
+    layer._stacked(torch.device("meta"))
+    assert len(made) == 3

@@ -5,6 +5,8 @@ Tolerances: products of two bf16 numbers are exact in f32; every addition of a s
 round, is off by at most a whole unit in the last place, 2^-23 of the sum of the magnitudes; a rounding to bf16 by half a step, 2^-8 of
 the value.
 """
+import weakref
+
 import pytest
 import torch
 
@@ -107,3 +109,26 @@ def test_biases_of_compressed_experts_that_train_get_their_gradient(int8, of_x):
         assert torch.equal(grads[experts], want)
     with torch.no_grad():
         assert torch.equal(layer(x, plan), frozen)
+
+
+def test_a_mixture_on_the_host_plans_once_and_one_that_leaves_the_device_lets_go():
+    experts, outer, inner, tokens = 3, 72, 128, 40
+    layer = ep.CompressedGroupedLinear.from_linears(_linears(experts, outer, inner), config=ep.EntroPackLossyConfig(target_bpp=4.0))
+    plan = ep.group_rows(torch.arange(tokens, device="cuda") % (experts + 1), experts)
+    x = torch.randn(tokens, inner, device="cuda").bfloat16()
+    there = layer(x, plan)
+    held = layer._decoder
+    assert torch.equal(layer(x, plan), there) and layer._decoder is held
+    leaf = x.clone().requires_grad_(True)
+    layer(leaf, plan).sum().backward()
+    assert layer._decoder is held
+    layer.cuda()
+    assert layer._decoder is None and torch.equal(layer(x, plan), there)
+    again = layer._decoder
+    assert torch.equal(layer.dequantize("cuda"), layer.dequantize()) and layer._decoder is again
+    del again
+    payload = weakref.ref(layer.experts[0].weight.buffers["payload"])
+    del held
+    layer.cpu()
+    assert payload() is None
+    assert torch.equal(layer(x, plan), there)
