@@ -18,7 +18,7 @@ from ..backends import hip as _hip
 from ..compression import BatchDecompressor
 from . import kernels
 from .groups import MAX_GROUPS, RowGroups, device_of, first_order, matrix, refuse_tangents, rows_of, sum_entries
-from .linear import CompressedINT8Linear, CompressedLinear
+from .linear import FORWARD_MODES, CompressedINT8Linear, CompressedLinear
 
 
 def _check_groups(name: str, x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bias, x_grouped: bool) -> None:
@@ -195,7 +195,8 @@ class CompressedGroupedLinear(torch.nn.Module):
     """The same projection of every expert of a mixture, each expert's weight compressed in a layer of its own.
 
     `experts`: `CompressedLinear` layers (bf16 containers) or `CompressedINT8Linear` layers, one class, one shape, with
-    biases in all of them or in none. They stay ordinary submodules: `state_dict` holds `experts.<i>.weight.entropack_quant_state`
+    biases in all of them or in none, with the default `forward_mode` and no `DecodeAhead` attached (this layer decodes and multiplies by
+    itself, and would use neither). They stay ordinary submodules: `state_dict` holds `experts.<i>.weight.entropack_quant_state`
     and so on. A forward decodes all experts (in one pass when their weights are `lattice_rans` containers), then runs
     `grouped_linear` or, for int8 experts, the row quantiser and `grouped_int8_linear`. Differentiable in x and in the biases (which the
     layers keep frozen unless asked otherwise). The first forward
@@ -226,6 +227,7 @@ class CompressedGroupedLinear(torch.nn.Module):
                 raise ValueError("the experts' rotation groups differ")
         self.experts = torch.nn.ModuleList(experts)
         self.in_features, self.out_features = first.in_features, first.out_features
+        self._check_settings()
         self._int8 = kind is CompressedINT8Linear
         self._decoder = None            # (device, the experts' payloads it was planned for, BatchDecompressor)
 
@@ -251,8 +253,17 @@ class CompressedGroupedLinear(torch.nn.Module):
     def groups(self) -> int:
         return len(self.experts)
 
+    def _check_settings(self) -> None:
+        """Refuses experts that were told to work in another way than this layer does."""
+        for expert in self.experts:
+            if expert.forward_mode != FORWARD_MODES[0]:
+                raise ValueError(f"CompressedGroupedLinear decodes its experts and multiplies, forward_mode {FORWARD_MODES[0]!r}, got an expert with {expert.forward_mode!r}")
+            if expert._decode_ahead is not None:
+                raise ValueError("CompressedGroupedLinear decodes its experts by itself, got one that is attached to a DecodeAhead: close that first")
+
     def _stacked(self, device: torch.device) -> torch.Tensor:
         """All experts' containers decoded: [experts, out_features, in_features] in the containers' dtype."""
+        self._check_settings()
         containers = [expert._container() for expert in self.experts]
         if any(container.compress_method != "lattice_rans" for container in containers):
             return torch.stack([expert.codes(device) if self._int8 else expert.dequantize(device).to(expert.container_dtype) for expert in self.experts])

@@ -158,3 +158,22 @@ def test_a_mixture_plans_once_wherever_its_containers_are(monkeypatch):
     layer._stacked(torch.device("meta"))
     layer._stacked(torch.device("meta"))
     assert len(made) == 3
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+def test_a_mixture_refuses_experts_with_settings_that_it_would_not_follow(int8):
+    kind = ep.CompressedINT8Linear if int8 else ep.CompressedLinear
+    for mode in ("fused", "fused_through_lds"):
+        with pytest.raises(ValueError, match="forward_mode"):
+            ep.CompressedGroupedLinear([kind(16, 8), kind(16, 8, forward_mode=mode)])
+    attached = kind(16, 8)
+    attached._decode_ahead = object()
+    with pytest.raises(ValueError, match="DecodeAhead"):
+        ep.CompressedGroupedLinear([kind(16, 8), attached])
+    layer = ep.CompressedGroupedLinear([kind(16, 8) for _ in range(2)])               # set afterwards: the forward refuses
+    layer.experts[1].forward_mode = "fused"
+    with pytest.raises(ValueError, match="forward_mode"):
+        layer.dequantize() if not int8 else layer._stacked(torch.device("cpu"))
+    layer.experts[1].forward_mode, layer.experts[0]._decode_ahead = "decode_then_gemm", object()
+    with pytest.raises(ValueError, match="DecodeAhead"):
+        layer._stacked(torch.device("cpu"))
