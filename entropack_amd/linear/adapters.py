@@ -72,7 +72,7 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
         x: bf16 [tokens, in_features], its input.
         down: bf16 [adapters, rank, in_features]. up: bf16 [adapters, out_features, rank].
         groups: the plan of `group_rows(ids, adapters)` with one id per token.
-        scale: f32 [adapters] or None for ones; it gets no gradient.
+        scale: f32 [adapters] or None for ones; it gets no gradient, and one that wants it is refused while gradients are recorded.
 
     Sums and the narrow rows between the two products are f32; the result is rounded to bf16 once. An infinity or NaN in a row's adapter makes that row's results NaN where it reaches them. Differentiable in y, x, down and
     up, in reverse mode.
@@ -98,7 +98,7 @@ def low_rank_update(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: to
     if scale is not None:
         if tuple(scale.shape) != (groups.groups,):
             raise ValueError(f"low_rank_update takes one scale per adapter, got shape {tuple(scale.shape)}")
-        if scale.requires_grad:
+        if scale.requires_grad and torch.is_grad_enabled():
             raise ValueError("low_rank_update gives no gradient of the scale: detach it")
         scale = scale if scale.dtype == torch.float32 and scale.is_contiguous() else scale.float().contiguous()
     device_of("low_rank_update", y, x, down, up, groups.order, scale)

@@ -148,6 +148,8 @@ def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups
         weight: int8 [groups, out_features, in_features].
         x_scale: f32, one per row of x. weight_scale: f32 [groups, out_features].
         bias: [groups, out_features] or None. out_dtype: bfloat16, float16 or float32.
+
+    Nothing gets a gradient; scales and biases that want one are refused while gradients are recorded.
     """
     _check_groups("grouped_int8_linear", x, weight, groups, bias, x_grouped)
     if x.dtype != torch.int8 or weight.dtype != torch.int8:
@@ -157,6 +159,9 @@ def grouped_int8_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups
     if x_scale.numel() != x.shape[0] or tuple(weight_scale.shape) != tuple(weight.shape[:2]):
         raise ValueError(f"grouped_int8_linear takes {x.shape[0]} activation scales and weight scales of shape {tuple(weight.shape[:2])}, "
                          f"got {tuple(x_scale.shape)} and {tuple(weight_scale.shape)}")
+    for name, tensor in (("x_scale", x_scale), ("weight_scale", weight_scale), ("bias", bias)):
+        if tensor is not None and tensor.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"grouped_int8_linear gives no gradient of {name}: detach it")
     device = device_of("grouped_int8_linear", x, weight, groups.order, x_scale, weight_scale, bias)
     refuse_tangents("grouped_int8_linear", x_scale, weight_scale, bias)
     outer = weight.shape[1]

@@ -177,3 +177,18 @@ def test_a_mixture_refuses_experts_with_settings_that_it_would_not_follow(int8):
     layer.experts[1].forward_mode, layer.experts[0]._decode_ahead = "decode_then_gemm", object()
     with pytest.raises(ValueError, match="DecodeAhead"):
         layer._stacked(torch.device("cpu"))
+
+
+def test_operands_whose_gradient_is_not_given_are_refused_only_while_gradients_are_recorded(no_device):
+    name, run, operands = OPERATORS[4]
+    for which in range(len(operands)):
+        leaf = operands[which].clone().requires_grad_(True)
+        with pytest.raises(ValueError, match="gives no gradient"):
+            run(*[leaf if i == which else o for i, o in enumerate(operands)])
+        with torch.no_grad():
+            assert run(*[leaf if i == which else o for i, o in enumerate(operands)]).shape == (6, 5)
+    scaled = lambda s: OPERATORS[3][1](s)
+    with pytest.raises(ValueError, match="gives no gradient"):
+        scaled(torch.ones(4, requires_grad=True))
+    with torch.no_grad():
+        assert scaled(torch.ones(4, requires_grad=True)).shape == (3, 10)
