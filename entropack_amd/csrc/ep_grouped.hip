@@ -81,7 +81,7 @@ static int current_compute_units(int& units) {
 template <bool INT8, int MODE, bool GATHER = true>
 static int launch_tile(TileArgs t, int64_t row_tiles, int tile, hipStream_t s) {
   const int64_t blocks = tile == kWideTile ? wide_blocks(row_tiles, t.columns, t.compute_units) : row_tiles * ((t.columns + kTile - 1) / kTile);
-  if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+  if (!launch_fits(blocks, kTileThreads)) return EP_HIP_EUNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
   const bool whole = t.inner % 256 == 0 && (MODE == kForward || t.columns % tile == 0);
   constexpr bool kAlways = MODE == kGradWeight;             // a group's rows are of any number
@@ -255,6 +255,7 @@ int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int3
   if (dy_dev == nullptr || offsets_dev == nullptr || out_dev == nullptr || groups <= 0 || N <= 0 || N > 0x7FFFFFFF / groups || lddy < N || !kind_valid(out_kind))
     return EP_HIP_EINVAL;
   const int64_t blocks = groups * ((N + kSumColumns - 1) / kSumColumns);
+  if (!launch_fits(blocks, 64 * kSumWaves)) return EP_HIP_EUNSUPPORTED;
   const bool pairs = reinterpret_cast<uintptr_t>(dy_dev) % 4 == 0 && lddy % 2 == 0 && N % 2 == 0;
   hipLaunchKernelGGL(grouped_column_sums_kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kSumWaves), 0, static_cast<hipStream_t>(stream),
                      static_cast<const uint16_t*>(dy_dev), lddy, offsets_dev, static_cast<int>(N), out_dev, out_kind, pairs ? 1 : 0);

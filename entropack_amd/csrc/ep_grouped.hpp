@@ -13,6 +13,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int64_t kMostEntries = int64_t{1} << 30;
 
+// A launch has fewer than 2^32 work items.
+inline bool launch_fits(int64_t blocks, int threads) { return blocks <= 0xFFFFFFFF / threads; }
+
 // What a lane loads whose piece lies past an operand's end.
 __device__ __align__(16) const uint32_t kZeroPiece[4] = {0, 0, 0, 0};
 
@@ -254,7 +257,7 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_stream_kernel(GroupedArgs 
 template <bool INT8, int MT, int NT, int WAVES, bool PLANES>
 static int launch_stream_of(const GroupedArgs& a, hipStream_t s) {
   const int64_t blocks = most_row_tiles(a.entries, a.groups, 16 * MT) * ((a.N + 16 * NT - 1) / (16 * NT));
-  if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+  if (!launch_fits(blocks, 64 * WAVES)) return EP_HIP_EUNSUPPORTED;
   hipLaunchKernelGGL((grouped_stream_kernel<INT8, MT, NT, WAVES, PLANES>), dim3(static_cast<unsigned>(blocks)), dim3(64 * WAVES), 0, s, a);
   EP_HIP_TRY(hipGetLastError());
   return EP_HIP_OK;

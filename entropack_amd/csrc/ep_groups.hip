@@ -351,6 +351,14 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const uint16_t* __res
   }
 }
 
+// Blocks of 256 threads in a launch (fewer than 2^32 work items): more tokens take several.
+constexpr int64_t kMostBlocks = 0xFFFFFFFF / 256;
+
+// The weights from entry `entry` on, which may be absent.
+static const void* weights_from(const void* weight, int kind, int64_t entry) {
+  return weight != nullptr ? static_cast<const uint8_t*>(weight) + entry * (kind == kOutF32 ? 4 : 2) : nullptr;
+}
+
 static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace ep
@@ -386,23 +394,29 @@ int ep_hip_combine_rows(const void* y_dev, int y_kind, int64_t ldy, const int32_
   if ((y_kind != kOutBF16 && y_kind != kOutF32) || (weight_dev != nullptr && weight_kind != kOutBF16 && weight_kind != kOutF32)) return EP_HIP_EINVAL;
   if (tokens > kMostEntries / per_row) return EP_HIP_EUNSUPPORTED;
   const bool wide = width % 8 == 0 && ldy % 8 == 0 && ldo % 8 == 0 && aligned16(y_dev) && aligned16(out_dev);
-  const int64_t threads = tokens * (wide ? width / 8 : width);
-  if ((threads + 255) / 256 > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
+  const int64_t pieces = wide ? width / 8 : width, together = kMostBlocks * 256 / pieces;            // tokens per launch
   hipStream_t s = static_cast<hipStream_t>(stream);
-  uint16_t* out = static_cast<uint16_t*>(out_dev);
   const int w = static_cast<int>(width);
-#define EP_COMBINE(ROW, VEC) \
-  hipLaunchKernelGGL((combine_rows_kernel<ROW, VEC>), grid, dim3(256), 0, s, static_cast<const ROW*>(y_dev), ldy, place_dev, kept_rows_dev, weight_dev, weight_kind, per_row, tokens, w, out, ldo)
-  if (y_kind == kOutBF16) {
-    if (wide) EP_COMBINE(uint16_t, 8);
-    else EP_COMBINE(uint16_t, 1);
-  } else {
-    if (wide) EP_COMBINE(float, 8);
-    else EP_COMBINE(float, 1);
-  }
+  for (int64_t from = 0; from < tokens; from += together) {
+    const int64_t here = tokens - from < together ? tokens - from : together, entry = from * per_row;
+    const dim3 grid(static_cast<unsigned>((here * pieces + 255) / 256));
+    uint16_t* const out = static_cast<uint16_t*>(out_dev) + from * ldo;
+    const int32_t* const place = place_dev != nullptr ? place_dev + entry : nullptr;
+    const int64_t row = place_dev != nullptr ? 0 : entry;     // rows of y are found by their place, or lie in the order of the entries
+    const void* const weight = weights_from(weight_dev, weight_kind, entry);
+#define EP_COMBINE(ROW, VEC)                                                                                                                         \
+  hipLaunchKernelGGL((combine_rows_kernel<ROW, VEC>), grid, dim3(256), 0, s, static_cast<const ROW*>(y_dev) + row * ldy, ldy, place, kept_rows_dev, weight, \
+                     weight_kind, per_row, here, w, out, ldo)
+    if (y_kind == kOutBF16) {
+      if (wide) EP_COMBINE(uint16_t, 8);
+      else EP_COMBINE(uint16_t, 1);
+    } else {
+      if (wide) EP_COMBINE(float, 8);
+      else EP_COMBINE(float, 1);
+    }
 #undef EP_COMBINE
-  EP_HIP_TRY(hipGetLastError());
+    EP_HIP_TRY(hipGetLastError());
+  }
   return EP_HIP_OK;
 }
 
@@ -417,17 +431,22 @@ int ep_hip_combine_rows_grad(const void* grad_dev, int64_t ldg, const void* y_de
   if (tokens > kMostEntries / per_row) return EP_HIP_EUNSUPPORTED;
   const bool wide = width % 8 == 0 && ldg % 8 == 0 && aligned16(grad_dev) && (grad_weight_dev == nullptr || (ldy % 8 == 0 && aligned16(y_dev))) &&
                     (grad_y_dev == nullptr || (ldgy % 8 == 0 && aligned16(grad_y_dev)));
-  const dim3 grid(static_cast<unsigned>(tokens));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint16_t* grad = static_cast<const uint16_t*>(grad_dev);
   const uint16_t* y = static_cast<const uint16_t*>(y_dev);
   uint16_t* grad_y = static_cast<uint16_t*>(grad_y_dev);
   const int w = static_cast<int>(width);
-  if (wide)
-    hipLaunchKernelGGL(combine_grad_kernel<8>, grid, dim3(256), 0, s, grad, ldg, y, ldy, place_dev, kept_rows_dev, weight_dev, weight_kind, per_row, w, grad_y, ldgy, grad_weight_dev);
-  else
-    hipLaunchKernelGGL(combine_grad_kernel<1>, grid, dim3(256), 0, s, grad, ldg, y, ldy, place_dev, kept_rows_dev, weight_dev, weight_kind, per_row, w, grad_y, ldgy, grad_weight_dev);
-  EP_HIP_TRY(hipGetLastError());
+  for (int64_t from = 0; from < tokens; from += kMostBlocks) {               // a block per token
+    const dim3 grid(static_cast<unsigned>(tokens - from < kMostBlocks ? tokens - from : kMostBlocks));
+    const int64_t entry = from * per_row;
+    const uint16_t* const grad = static_cast<const uint16_t*>(grad_dev) + from * ldg;
+    const void* const weight = weights_from(weight_dev, weight_kind, entry);
+    void* const grad_weight = const_cast<void*>(weights_from(grad_weight_dev, weight_kind, entry));
+    if (wide)
+      hipLaunchKernelGGL(combine_grad_kernel<8>, grid, dim3(256), 0, s, grad, ldg, y, ldy, place_dev + entry, kept_rows_dev, weight, weight_kind, per_row, w, grad_y, ldgy, grad_weight);
+    else
+      hipLaunchKernelGGL(combine_grad_kernel<1>, grid, dim3(256), 0, s, grad, ldg, y, ldy, place_dev + entry, kept_rows_dev, weight, weight_kind, per_row, w, grad_y, ldgy, grad_weight);
+    EP_HIP_TRY(hipGetLastError());
+  }
   return EP_HIP_OK;
 }
 

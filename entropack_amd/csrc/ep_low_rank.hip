@@ -358,7 +358,7 @@ static int expand(const Grouping& g, const void* planes, const void* up, int64_t
   const bool tall = g.entries / g.groups >= 32;              // most blocks of 64 rows are then at least half full
   const int columns = tall ? kTallColumns : 256;
   const int64_t blocks = most_row_tiles(g.entries, g.groups, tall ? 64 : 16) * ((N + columns - 1) / columns);
-  if (blocks > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+  if (!launch_fits(blocks, 256)) return EP_HIP_EUNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks));
 #define EP_EXPAND(PIECES, WIDE)                                                                                               \
   if (!tall) hipLaunchKernelGGL((low_rank_expand_kernel<PIECES, WIDE>), grid, dim3(256), 0, s, a);                             \
@@ -411,7 +411,7 @@ static int reduce(const Grouping& g, int64_t rank, int chunk, const Reduction* a
     blocks[i] = most_chunks(g.entries, g.groups, chunk) * ((t.rows + kTile - 1) / kTile) * ((r.width + kTile - 1) / kTile);
     finish[i] = static_cast<int64_t>(g.groups) * (padded / 16) * ((r.width + 63) / 64);
   }
-  if (blocks[0] + blocks[1] > 0x7FFFFFFF || finish[0] + finish[1] > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+  if (!launch_fits(blocks[0] + blocks[1], kTileThreads) || !launch_fits(finish[0] + finish[1], 1024)) return EP_HIP_EUNSUPPORTED;
   hipLaunchKernelGGL(low_rank_reduce_kernel, dim3(static_cast<unsigned>(blocks[0] + blocks[1])), dim3(kTileThreads), 0, s, tiles[0], tiles[1], static_cast<int>(blocks[0]));
   EP_HIP_TRY(hipGetLastError());
   hipLaunchKernelGGL(low_rank_finish_kernel, dim3(static_cast<unsigned>(finish[0] + finish[1])), dim3(1024), 0, s, sums[0], sums[1], static_cast<int>(finish[0]), chunk, padded,
@@ -445,6 +445,9 @@ static bool low_rank_valid(const Grouping& g, int64_t rank, int64_t K, int64_t N
          K <= 0x3FFFFF00 / g.groups && N <= 0x3FFFFF00 / g.groups;
 }
 
+// The rows that one launch of the shrink takes, 16 per block of 256 threads: fewer than 2^28.
+static bool rows_fit(int64_t entries, int groups) { return launch_fits(most_row_tiles(entries, groups, 16), 256); }
+
 // Rows read in whole 16-byte pieces, the last one zero from `width` on.
 static bool rows_in_pieces(const void* base, int64_t ld, int64_t width) {
   return base != nullptr && reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld % 8 == 0 && ld >= whole_pieces(width);
@@ -464,6 +467,7 @@ int ep_hip_low_rank_update(const void* x_dev, int64_t ldx, const void* down_dev,
   if (!low_rank_valid(g, rank, K, N) || planes_dev == nullptr || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0) return EP_HIP_EINVAL;
   if (!rows_in_pieces(x_dev, ldx, K) || !rows_in_pieces(down_dev, ldd, K) || down_group % 8 != 0 || down_group < 0) return EP_HIP_EINVAL;
   if (up_dev == nullptr || out_dev == nullptr || ldu < rank || up_group < 0 || ldo < N || (y_dev != nullptr && ldy < N)) return EP_HIP_EINVAL;
+  if (!rows_fit(entries, groups)) return EP_HIP_EUNSUPPORTED;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int status = shrink(g, x_dev, ldx, down_dev, ldd, down_group, scale_dev, planes_dev, rank, whole_pieces(K), s);
   return status != EP_HIP_OK ? status : expand(g, planes_dev, up_dev, ldu, up_group, y_dev, ldy, out_dev, ldo, rank, N, s);
@@ -487,6 +491,7 @@ int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x
   if (grad_x_dev != nullptr && (down_dev == nullptr || ldd < K || down_group < 0 || ldgx < K)) return EP_HIP_EINVAL;
   if (grad_down_dev != nullptr && !rows_in_pieces(x_dev, ldx, K)) return EP_HIP_EINVAL;
   if (grad_up_dev != nullptr && (planes_dev == nullptr || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0)) return EP_HIP_EINVAL;
+  if (!rows_fit(entries, groups)) return EP_HIP_EUNSUPPORTED;
   const GradRoom room = grad_room(entries, groups, rank, K, N);
   if (workspace_dev == nullptr || reinterpret_cast<uintptr_t>(workspace_dev) % 256 != 0 || workspace_bytes < room.bytes) return EP_HIP_EINVAL;
   uint8_t* const base = static_cast<uint8_t*>(workspace_dev);
@@ -499,7 +504,7 @@ int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x
     Transpose down = {static_cast<const uint16_t*>(down_dev), reinterpret_cast<uint16_t*>(base + room.down_turned), ldd, down_group, static_cast<int>(rank), static_cast<int>(K),
                       static_cast<int>(whole_pieces(rank)), 0, 0};
     const int64_t first = tiles(up) * groups, second = tiles(down) * (grad_x_dev != nullptr ? groups : 0);
-    if (first + second > 0x7FFFFFFF) return EP_HIP_EUNSUPPORTED;
+    if (!launch_fits(first + second, 256)) return EP_HIP_EUNSUPPORTED;
     hipLaunchKernelGGL(low_rank_transpose_kernel, dim3(static_cast<unsigned>(first + second)), dim3(256), 0, s, up, down, static_cast<int>(first));
     EP_HIP_TRY(hipGetLastError());
     const int64_t turned = whole_pieces(N);

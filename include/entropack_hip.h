@@ -419,7 +419,8 @@ int ep_hip_tile_ans_encode(const uint8_t* bytes_dev, int64_t num_elements, int n
  * its id names its group, an id outside [0, groups) no group. `order` lists the entries sorted by group (entries of one group in
  * their own order, those of no group last), `offsets` (int32[groups + 1]) the first place of every group in that list,
  * `place` is the inverse of `order`. Rows "in grouped order" lie one per place. The products below take order, offsets,
- * place and rows as ep_hip_group_rows wrote them. At most 2^30 entries and 896 groups. */
+ * place and rows as ep_hip_group_rows wrote them. At most 2^30 entries and 896 groups; what would take more than 2^32 work items in one
+ * launch is refused as unsupported (adapters: somewhat below 2^28 rows). */
 
 /* ids_dev: int32 or int64 (id_bytes 4 or 8) [entries]; order_dev, place_dev: int32[entries]; offsets_dev: int32[groups + 1];
  * rows_dev (int32[entries], NULL when not wanted): the token of every place, order / per_row.

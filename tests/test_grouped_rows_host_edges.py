@@ -192,3 +192,17 @@ def test_operands_whose_gradient_is_not_given_are_refused_only_while_gradients_a
         scaled(torch.ones(4, requires_grad=True))
     with torch.no_grad():
         assert scaled(torch.ones(4, requires_grad=True)).shape == (3, 10)
+
+
+def test_launches_of_too_many_work_items_are_refused_before_they_are_made():
+    """A launch has fewer than 2^32 work items. Nothing is launched, so no device is needed and no address is followed."""
+    lib, at = hip.library(), 4096
+    update = lambda rows, count: lib.ep_hip_low_rank_update(at, 16, at, 16, 64, at, 4, 64, None, at, 16, at, at, 16, at, at, rows, count, 4, 16, 16, None)
+    grad = lambda rows, count: lib.ep_hip_low_rank_update_grad(at, 16, at, 16, at, 16, 64, at, 4, 64, None, at, at, 16, at, at, at, at, rows, count, 4, 16, 16, at, 1 << 62, None)
+    sums = lambda count, columns: lib.ep_hip_grouped_column_sums_bf16(at, columns, at, count, columns, at, 0, None)
+    for call in (update, grad):
+        for rows, count in ((1 << 30, 1), (1 << 28, 2), ((1 << 28) - 14000, 896)):
+            assert call(rows, count) == hip.EUNSUPPORTED
+    assert sums(1, 1 << 30) == hip.EUNSUPPORTED and sums(500, 1 << 21) == hip.EUNSUPPORTED
+    # 100 entries in 30 groups by 2^25 columns, 16 rows and 16 columns per block of 256 threads
+    assert lib.ep_hip_grouped_gemm_bf16(at, 16, 100, at, 16, 64, None, at, 1 << 25, 0, at, at, 100, 30, 1 << 25, 16, None) == hip.EUNSUPPORTED

@@ -132,3 +132,32 @@ def test_a_mixture_on_the_host_plans_once_and_one_that_leaves_the_device_lets_go
     layer.cpu()
     assert payload() is None
     assert torch.equal(layer(x, plan), there)
+
+
+@pytest.mark.parametrize("width", [8, 257], ids=["a block per token", "a thread per element"])
+def test_weighted_return_of_more_tokens_than_a_launch_takes(width):
+    """2^24 + 37 tokens: the gradient's blocks of one token each, and at width 257 the forward's threads too, pass 2^32 work items. One entry
+    per token and no weight: the return and its gradient copy rows, exactly. With weights: a power of two each, exact again."""
+    tokens, count = (1 << 24) + 37, 5
+    source = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.randint(-1, count, (tokens,), device="cuda", generator=source)
+    plan = ep.group_rows(ids, count)
+    place, none = plan.place.long(), ids < 0
+    y = torch.empty(tokens, width, dtype=torch.bfloat16, device="cuda").normal_(generator=source)
+    for weight in (None, torch.exp2(torch.randint(-3, 3, (tokens,), device="cuda", generator=source).float())):
+        leaves = [y.requires_grad_(True)] + ([] if weight is None else [weight.requires_grad_(True)])
+        out = ep.combine_rows(y, plan, weight)
+        dout = torch.empty_like(out).normal_(generator=source)
+        grads = torch.autograd.grad(out, leaves, dout)
+        with torch.no_grad():
+            for first in range(0, tokens, 1 << 21):
+                some = slice(first, first + (1 << 21))
+                factor = 1.0 if weight is None else weight[some].unsqueeze(1)
+                dead = none[some].unsqueeze(1)
+                rows = y[place[some]].float()
+                assert torch.equal(out[some], torch.where(dead, 0.0, factor * rows).bfloat16())
+                assert torch.equal(grads[0][place[some]], torch.where(dead, 0.0, factor * dout[some].float()).bfloat16())
+                if weight is not None:
+                    dot, size = (rows.double() * dout[some].double()).sum(1), (rows.double() * dout[some].double()).abs().sum(1)
+                    _within(grads[1][some], torch.where(none[some], 0.0, dot), (width + 2) * STEP_F32 * size)
+        del out, dout, grads
