@@ -189,6 +189,8 @@ _SIGNATURES = {
         ctypes.c_void_p]),
     "ep_hip_low_rank_grad_workspace": (ctypes.c_size_t, [
         ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]),
+    "ep_hip_low_rank_grad_workspace_for": (ctypes.c_size_t, [
+        ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "ep_hip_low_rank_update_grad": (ctypes.c_int, [
         ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,

@@ -420,23 +420,35 @@ static int reduce(const Grouping& g, int64_t rank, int chunk, const Reduction* a
   return EP_HIP_OK;
 }
 
-// Where the gradients keep what lies between their products: both transposes, the planes of the output's gradient, the chunks' sums of
-// both.
+// Which gradients a call gives.
+enum : int { kWantX = 1, kWantDown = 2, kWantUp = 4, kWantAll = 7 };
+
+// Where they keep what lies between their products, each part only where a gradient asked for reads it: the transpose of up and the
+// planes of the output's gradient (of x and of down), the transpose of down (of x), the chunks' sums (of down, of up). The chunks' sums
+// are f32 matrices, one per chunk, and a group with places has a chunk at least: up to twice the gradients' own size for a bank whose
+// adapters all have rows. The chunks do not depend on what is asked for, so neither do the sums' values.
 struct GradRoom {
   size_t up_turned, down_turned, planes, down_parts, up_parts, bytes;
   int chunk;
 };
 
-static GradRoom grad_room(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N) {
-  GradRoom r;
+static GradRoom grad_room(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N, int wanted) {
+  GradRoom r = {};
   const size_t g = static_cast<size_t>(groups);
-  r.up_turned = 0;                                                                         // [groups][rank][whole pieces of N]
-  r.down_turned = r.up_turned + whole_lines(g * static_cast<size_t>(rank * whole_pieces(N)) * 2);     // [groups][K][whole pieces of rank]
-  r.planes = r.down_turned + whole_lines(g * static_cast<size_t>(K * whole_pieces(rank)) * 2);
+  size_t end = 0;
+  auto take = [&](bool needed, size_t bytes) {
+    const size_t at = end;
+    if (needed) end += whole_lines(bytes);
+    return at;
+  };
+  const bool back = (wanted & (kWantX | kWantDown)) != 0;
   r.chunk = reduce_chunk(entries, rank, K, N);
-  r.down_parts = r.planes + whole_lines(planes_bytes(entries, rank));
-  r.up_parts = r.down_parts + whole_lines(reduce_bytes(entries, groups, rank, r.chunk, K));
-  r.bytes = r.up_parts + reduce_bytes(entries, groups, rank, r.chunk, N);
+  r.up_turned = take(back, g * static_cast<size_t>(rank * whole_pieces(N)) * 2);                       // [groups][rank][whole pieces of N]
+  r.down_turned = take((wanted & kWantX) != 0, g * static_cast<size_t>(K * whole_pieces(rank)) * 2);     // [groups][K][whole pieces of rank]
+  r.planes = take(back, planes_bytes(entries, rank));
+  r.down_parts = take((wanted & kWantDown) != 0, reduce_bytes(entries, groups, rank, r.chunk, K));
+  r.up_parts = take((wanted & kWantUp) != 0, reduce_bytes(entries, groups, rank, r.chunk, N));
+  r.bytes = end;
   return r;
 }
 
@@ -475,7 +487,13 @@ int ep_hip_low_rank_update(const void* x_dev, int64_t ldx, const void* down_dev,
 
 size_t ep_hip_low_rank_grad_workspace(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N) {
   if (entries <= 0 || groups <= 0 || rank <= 0 || K <= 0 || N <= 0) return 0;
-  return ep::grad_room(entries, groups, rank, K, N).bytes;
+  return ep::grad_room(entries, groups, rank, K, N, ep::kWantAll).bytes;
+}
+
+size_t ep_hip_low_rank_grad_workspace_for(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N, int grad_x, int grad_down, int grad_up) {
+  using namespace ep;
+  if (entries <= 0 || groups <= 0 || rank <= 0 || K <= 0 || N <= 0) return 0;
+  return grad_room(entries, groups, rank, K, N, (grad_x != 0 ? kWantX : 0) | (grad_down != 0 ? kWantDown : 0) | (grad_up != 0 ? kWantUp : 0)).bytes;
 }
 
 int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group,
@@ -492,7 +510,7 @@ int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x
   if (grad_down_dev != nullptr && !rows_in_pieces(x_dev, ldx, K)) return EP_HIP_EINVAL;
   if (grad_up_dev != nullptr && (planes_dev == nullptr || reinterpret_cast<uintptr_t>(planes_dev) % 16 != 0)) return EP_HIP_EINVAL;
   if (!rows_fit(entries, groups)) return EP_HIP_EUNSUPPORTED;
-  const GradRoom room = grad_room(entries, groups, rank, K, N);
+  const GradRoom room = grad_room(entries, groups, rank, K, N, (grad_x_dev != nullptr ? kWantX : 0) | (grad_down_dev != nullptr ? kWantDown : 0) | (grad_up_dev != nullptr ? kWantUp : 0));
   if (workspace_dev == nullptr || reinterpret_cast<uintptr_t>(workspace_dev) % 256 != 0 || workspace_bytes < room.bytes) return EP_HIP_EINVAL;
   uint8_t* const base = static_cast<uint8_t*>(workspace_dev);
   hipStream_t s = static_cast<hipStream_t>(stream);

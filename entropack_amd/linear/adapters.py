@@ -50,7 +50,7 @@ class _LowRankUpdate(torch.autograd.Function):
         grad_x = torch.empty(groups.entries, inner, dtype=torch.bfloat16, device=device) if need_x else None
         grad_down = torch.empty(adapters, rank, inner, dtype=torch.bfloat16, device=device) if need_down else None
         grad_up = torch.empty(adapters, outer, rank, dtype=torch.bfloat16, device=device) if need_up else None
-        room = _hip.library().ep_hip_low_rank_grad_workspace(groups.entries, adapters, rank, inner, outer)
+        room = _hip.library().ep_hip_low_rank_grad_workspace_for(groups.entries, adapters, rank, inner, outer, need_x, need_down, need_up)
         workspace = torch.empty(room, dtype=torch.uint8, device=device)
         slope = matrix(grad, 8)
         _hip.launch("ep_hip_low_rank_update_grad", device,

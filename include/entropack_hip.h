@@ -472,12 +472,16 @@ int ep_hip_grouped_column_sums_bf16(const void* dy_dev, int64_t lddy, const int3
  * what then remains, 16 zeros. The gradient of up reads them.
  * _grad: any of grad_x [entries][K] (rows of no adapter zero), grad_down [groups][rank][K] and grad_up [groups][N][rank] (contiguous),
  * each absent when NULL, from grad_dev, the output's gradient [entries][N], read in whole pieces as x is; up is needed for the
- * first two, down for the first, x for the second, planes (of the forward) for the third. workspace: 256-byte aligned. */
+ * first two, down for the first, x for the second, planes (of the forward) for the third. workspace: 256-byte aligned, of
+ * ep_hip_low_rank_grad_workspace bytes for any of them or of ep_hip_low_rank_grad_workspace_for (non-zero: wanted) for those a call asks
+ * for. grad_down and grad_up each take an f32 matrix per chunk of places, at most min(groups, entries) of them and a number that grows with the
+ * entries: up to twice the size of the gradients themselves for a bank of many adapters. */
 size_t ep_hip_low_rank_planes_bytes(int64_t entries, int64_t rank);
 int ep_hip_low_rank_update(const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group, const void* up_dev, int64_t ldu, int64_t up_group,
                            const float* scale_dev, const void* y_dev, int64_t ldy, void* planes_dev, void* out_dev, int64_t ldo, const int32_t* order_dev,
                            const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank, int64_t K, int64_t N, void* stream);
 size_t ep_hip_low_rank_grad_workspace(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N);
+size_t ep_hip_low_rank_grad_workspace_for(int64_t entries, int groups, int64_t rank, int64_t K, int64_t N, int grad_x, int grad_down, int grad_up);
 int ep_hip_low_rank_update_grad(const void* grad_dev, int64_t ldg, const void* x_dev, int64_t ldx, const void* down_dev, int64_t ldd, int64_t down_group,
                                 const void* up_dev, int64_t ldu, int64_t up_group, const float* scale_dev, const void* planes_dev, void* grad_x_dev, int64_t ldgx,
                                 void* grad_down_dev, void* grad_up_dev, const int32_t* order_dev, const int32_t* offsets_dev, int64_t entries, int groups, int64_t rank,

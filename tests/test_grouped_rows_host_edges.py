@@ -206,3 +206,25 @@ def test_launches_of_too_many_work_items_are_refused_before_they_are_made():
     assert sums(1, 1 << 30) == hip.EUNSUPPORTED and sums(500, 1 << 21) == hip.EUNSUPPORTED
     # 100 entries in 30 groups by 2^25 columns, 16 rows and 16 columns per block of 256 threads
     assert lib.ep_hip_grouped_gemm_bf16(at, 16, 100, at, 16, 64, None, at, 1 << 25, 0, at, at, 100, 30, 1 << 25, 16, None) == hip.EUNSUPPORTED
+
+
+@pytest.mark.parametrize("entries,count,rank,inner,outer", [(1024, 64, 64, 8192, 8192), (1000, 896, 64, 4096, 4096), (7, 3, 5, 72, 40), (5000, 2, 16, 4096, 1024)])
+def test_workspace_of_the_adapters_gradients_holds_what_is_asked_for(entries, count, rank, inner, outer):
+    room = lambda *wanted: hip.library().ep_hip_low_rank_grad_workspace_for(entries, count, rank, inner, outer, *wanted)
+    line = 256
+    whole = lambda n, unit: -(-n // unit) * unit
+    turned_up, turned_down = 2 * count * rank * whole(outer, 8), 2 * count * inner * whole(rank, 8)
+    planes = entries * whole(rank, 16) * 8
+    assert room(1, 0, 0) <= turned_up + turned_down + planes + 3 * line                # nothing of the weights' gradients
+    down_parts, up_parts = room(0, 1, 0) - room(1, 0, 0) + whole(turned_down, line), room(0, 0, 1)
+    assert room(0, 1, 0) == whole(turned_up, line) + whole(planes, line) + down_parts
+    assert room(1, 1, 1) == room(1, 0, 0) + down_parts + up_parts == hip.library().ep_hip_low_rank_grad_workspace(entries, count, rank, inner, outer)
+    assert room(0, 0, 0) == 0
+    # The sums: an f32 matrix per chunk of 128 places or more, one at least for every adapter with places.
+    chunks = min(count, entries) + entries // 128
+    assert up_parts <= 4 * chunks * whole(rank, 16) * outer + line and down_parts <= 4 * chunks * whole(rank, 16) * inner + line
+    at = 4096
+    for gx, gd, gu in ((at, None, None), (None, at, None), (None, None, at), (at, at, None)):
+        wanted = [int(p is not None) for p in (gx, gd, gu)]
+        assert hip.library().ep_hip_low_rank_update_grad(at, whole(outer, 8), at, whole(inner, 8), at, whole(inner, 8), 0, at, rank, 0, None, at, gx, inner, gd, gu, at, at, entries, count,
+                                                         rank, inner, outer, at, room(*wanted) - 1, None) == hip.EINVAL

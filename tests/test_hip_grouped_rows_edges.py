@@ -11,9 +11,15 @@ import pytest
 import torch
 
 import entropack_amd as ep
+from entropack_amd.backends import hip
 
 pytestmark = pytest.mark.gpu
 HALF_BF16, STEP_F32 = 2.0 ** -8, 2.0 ** -23
+
+
+def whole(columns):
+    """Columns of a row in whole pieces of 16 bytes."""
+    return (columns + 7) // 8 * 8
 
 
 def _within(got, expect, bound):
@@ -161,3 +167,33 @@ def test_weighted_return_of_more_tokens_than_a_launch_takes(width):
                     dot, size = (rows.double() * dout[some].double()).sum(1), (rows.double() * dout[some].double()).abs().sum(1)
                     _within(grads[1][some], torch.where(none[some], 0.0, dot), (width + 2) * STEP_F32 * size)
         del out, dout, grads
+
+
+@pytest.mark.parametrize("wanted", range(1, 8))
+@pytest.mark.parametrize("tokens,count,rank,inner,outer", [(50, 3, 5, 72, 40), (700, 20, 33, 264, 130)])
+def test_gradients_of_adapters_keep_to_the_workspace_of_what_is_asked_for(wanted, tokens, count, rank, inner, outer):
+    """The entry point itself, its workspace between two guards and full of NaN, so that nothing can be read that was not written."""
+    lib = hip.library()
+    source = torch.Generator(device="cuda").manual_seed(2)
+    make = lambda *shape: torch.randn(*shape, device="cuda", generator=source).bfloat16()
+    plan = ep.group_rows(torch.randint(-1, count, (tokens,), device="cuda", generator=source), count)
+    y, x, down, up, dout = make(tokens, outer), make(tokens, inner), make(count, rank, inner), make(count, outer, rank), make(tokens, whole(outer))
+    dout[:, outer:] = 0
+    leaves = [t.requires_grad_(True) for t in (x, down, up)]
+    want = torch.autograd.grad(ep.low_rank_update(y, *leaves, plan), leaves, dout[:, :outer])
+    x, down, up = (t.detach() for t in leaves)
+    stream = torch.cuda.current_stream().cuda_stream
+    planes = torch.empty(lib.ep_hip_low_rank_planes_bytes(tokens, rank), dtype=torch.uint8, device="cuda")
+    out = torch.empty(tokens, outer, dtype=torch.bfloat16, device="cuda")
+    shape = (plan.order.data_ptr(), plan.offsets.data_ptr(), tokens, count, rank, inner, outer)
+    hip.check("forward", lib.ep_hip_low_rank_update(x.data_ptr(), inner, down.data_ptr(), inner, rank * inner, up.data_ptr(), rank, outer * rank, None, y.data_ptr(), outer, planes.data_ptr(),
+                                                    out.data_ptr(), outer, *shape, stream))
+    flags = [wanted & 1, wanted >> 1 & 1, wanted >> 2 & 1]
+    room, guard = lib.ep_hip_low_rank_grad_workspace_for(tokens, count, rank, inner, outer, *flags), 4096
+    space = torch.full((room + 2 * guard,), 0xFF, dtype=torch.uint8, device="cuda")
+    got = [torch.full_like(t, float("nan")) if flag else None for t, flag in zip((x, down, up), flags)]
+    at = [None if t is None else t.data_ptr() for t in got]
+    hip.check("gradients", lib.ep_hip_low_rank_update_grad(dout.data_ptr(), dout.stride(0), x.data_ptr(), inner, down.data_ptr(), inner, rank * inner, up.data_ptr(), rank, outer * rank, None,
+                                                           planes.data_ptr(), at[0], inner, at[1], at[2], *shape, space.data_ptr() + guard, room, stream))
+    assert space[:guard].eq(0xFF).all() and space[guard + room:].eq(0xFF).all()
+    assert all(torch.equal(a, b) for a, b, flag in zip(got, want, flags) if flag)
