@@ -163,6 +163,15 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
         const int cell = tid + 256 * m, column = first_column + cell / kPieces;
         moved[m] = up_piece<PIECES>(up + (column < a.N ? column : a.N - 1) * a.ldu, rank0 + 8 * (cell % kPieces), a.rank);
       }
+      // 16 ranks each: values and remainders (quarters 0, 1 and 2, 3), then last parts and zeros. Asked for with `up`; past the end the first again.
+      const int ranks = a.padded - rank0 < STEP ? a.padded - rank0 : STEP;
+      bf16x8 narrow[STEP / 16][2];
+#pragma unroll
+      for (int i = 0; i < STEP / 16; ++i) {
+        const uint16_t* from = planes + 4 * (rank0 + (16 * i < ranks ? 16 * i : 0));
+        narrow[i][0] = *reinterpret_cast<const bf16x8*>(from);
+        narrow[i][1] = *reinterpret_cast<const bf16x8*>(from + 32);
+      }
       if (rank0 > 0) __syncthreads();                        // the stretch before has been read
 #pragma unroll
       for (int m = 0; m < kMoves; ++m) {
@@ -170,16 +179,14 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
         *reinterpret_cast<uint4*>(up_tile + ((column & 7) * 16 + (column >> 3)) * kPitch + 16 * (cell % kPieces)) = moved[m];
       }
       __syncthreads();
-      const int ranks = a.padded - rank0 < STEP ? a.padded - rank0 : STEP;
-      // 16 ranks at a time: values and remainders (quarters 0, 1 and 2, 3), then last parts and zeros, both against the same `up`.
-      for (int e0 = 0; e0 < ranks; e0 += 16) {
-        const bf16x8 fp = *reinterpret_cast<const bf16x8*>(planes + 4 * (rank0 + e0));
-        const bf16x8 last = *reinterpret_cast<const bf16x8*>(planes + 4 * (rank0 + e0) + 32);
+#pragma unroll
+      for (int i = 0; i < STEP / 16; ++i) {
+        if (16 * i >= ranks) continue;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bf16x8 fu = *reinterpret_cast<const bf16x8*>(up_tile + (16 * j + in_row) * kPitch + 2 * (e0 + 8 * (quarter & 1)));
-          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(last, fu, acc[j], 0, 0, 0);
-          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp, fu, acc[j], 0, 0, 0);
+          const bf16x8 fu = *reinterpret_cast<const bf16x8*>(up_tile + (16 * j + in_row) * kPitch + 2 * (16 * i + 8 * (quarter & 1)));
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(narrow[i][1], fu, acc[j], 0, 0, 0);
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(narrow[i][0], fu, acc[j], 0, 0, 0);
         }
       }
     }
