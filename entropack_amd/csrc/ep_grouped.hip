@@ -143,8 +143,9 @@ __global__ __launch_bounds__(256) void grouped_sum_chunks_kernel(const float* __
 
 template <bool INT8>
 static int launch_grouped(const GroupedArgs& a, hipStream_t s) {
-  // Few rows per group: the weights' stream (MI355X, weights from memory). About one row per group: blocks of 16 weight rows; one token,
-  // two of eight experts 4096 x 4096, 12.7 us (floor 10.2), 18 tokens, four of 64 experts 1408 x 2048, 31.1 us. From five rows on
+  // Few rows per group: the weights' stream. About one row per group: blocks of 16 weight rows; one token, two of eight experts 4096 x
+  // 4096, 13.2 us (67 MB, 10.8 us at 6.2 TB/s) and 14.6 in int8, which the host's call bounds; 18 tokens, four of 64 experts 1408 x 2048, 31
+  // us with the weights partly in the last-level cache, 56 from memory (243 MB, 4.3 TB/s), 33 in int8. From five rows on
   // 32 rows by 32 weight rows (64 tokens, two of eight, 62 us; 256 tokens, four of 64, 75), from 24 on by 64 (128 tokens, two of
   // eight, 61 us against 73; 512 tokens, four of 64, 98 against 96). From 48 on the 128 x 128 tiles: 256 tokens, two of eight, 82 us
   // against 91; 1024 tokens, four of 64, 106 against 135.

@@ -56,7 +56,7 @@ __device__ __forceinline__ uint4 add_to_pieces(uint4 in, const f32x4& first, con
 // Few rows per adapter: a block takes 16 rows of one adapter and 256 columns, a wave 64 of them. The matrix cores are given the rows
 // of `up` as the left operand, ordered so that a lane ends up with two runs of 8 consecutive columns of its row (row m of tile j
 // is column 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4 of the 64). The inner dimension is [value | remainder] and [last part | zeros] of
-// 16 ranks, all against the same `up`. There is no LDS and nothing to wait for but the loads: 61 rows of 48 adapters take 3.5 us.
+// 16 ranks, all against the same `up`. There is no LDS and nothing to wait for but the loads: 61 rows of 48 adapters take 3.6 us.
 template <bool PIECES, bool WIDE>
 __global__ __launch_bounds__(256) void low_rank_expand_kernel(LowRankArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -118,11 +118,13 @@ __global__ __launch_bounds__(256) void low_rank_expand_kernel(LowRankArgs a) {
 
 // Many rows per adapter: bound by reading y and writing out. A block takes 64 rows of one adapter, 16 per wave, and 128 columns.
 // Memory wants neighbouring lanes at neighbouring addresses (a load whose lanes are on sixteen rows, as the fragments of the kernel
-// above are, occupies the address path four times as long: 7993 rows of 4096, rank 32, 46 us with it). So `up` goes through LDS,
+// above are, occupies the address path four times as long). So `up` goes through LDS,
 // STEP ranks at a time, fetched once for all 64 rows, and the planes are the left operand: lane l then holds, over the eight
 // 16-column tiles (row m of tile j is column 8 m + j), 8 consecutive columns 8 (l % 16) .. of rows 4 (l / 16) + i: sixteen lanes
-// read and write 256 consecutive bytes of a row. Small blocks, so that many are resident and the last round is short: 34 us
-// (256 columns per block 41, 512 columns 44; a copy of the same bytes 21).
+// read and write 256 consecutive bytes of a row. Small blocks, so that many are resident and the last round is short (256 columns per block
+// took a fifth more, 512 columns 30 %). The narrow rows' fragments are asked for with `up`, before the barrier, so that both arrive
+// together: 7993 rows of 4096, rank 32, 26.6 us, 31.8 with the fragments loaded where they are used (131 MB, 21 us at the rate of a large
+// read and write; a part of y comes from the last-level cache where a call is repeated).
 // STEP: the least of 16, 32 and 64 that the rank fits, 64 beyond.
 constexpr int kTallColumns = 128;
 
@@ -215,8 +217,8 @@ __global__ __launch_bounds__(256) void low_rank_expand_tall_kernel(LowRankArgs a
 // into one where the tile is stored. They are bound by
 // reading q, and the groups alone make too few tiles to fill the card, so the places of every group are divided into chunks, each
 // chunk writes its f32 sums to a matrix of its own, and this kernel adds a group's chunks in their order and rounds once.
-// A block takes 64 columns and 16 ranks of one group, a wave one of the ranks; bound by the latency of its loads: 36 chunks of rank 16
-// and 4096 columns, 4.4 us (4 waves with four ranks each 10.8); both gradients of 4 adapters, 4099 rows, 5.4 us. One launch sums both gradients, as one launch of tiles makes their parts:
+// A block takes 64 columns and 16 ranks of one group, a wave one of the ranks; bound by the latency of its loads: both gradients of 4
+// adapters of rank 16, 4099 rows of 4096, 5.2 us (4 waves with four ranks each take twice as long). One launch sums both gradients, as one launch of tiles makes their parts:
 // the blocks of the first before those of the second.
 struct Finish {
   const float* parts;
@@ -259,7 +261,8 @@ __global__ __launch_bounds__(1024) void low_rank_finish_kernel(Finish of_first, 
 }
 
 // The parts of both gradients, tiles of 128 x 128: the blocks of the first before those of the second. 4 adapters of rank 16, 4099 rows
-// of 4096 on either side, 21.7 us (a launch each, 16.5 and 16.5; reading both sides takes 11).
+// of 4096 on either side, 20 us (reading both sides takes 11). Ranks to 32 fit one tile of rows; rank 64 takes two, each of which reads the other
+// operand: 2 adapters, 20000 rows of 8192, 222 us (reading both sides 106).
 __global__ __launch_bounds__(kTileThreads, 2) void low_rank_reduce_kernel(TileArgs of_first, TileArgs of_second, int first_blocks) {
   __shared__ __align__(1024) uint8_t stage0[2 * kTile * 128];
   __shared__ __align__(1024) uint8_t stage1[2 * kTile * 128];
