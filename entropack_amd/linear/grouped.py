@@ -84,15 +84,14 @@ def _grad_weight(grad, x, weight, groups: RowGroups, x_grouped: bool) -> torch.T
     return out if tuple(out.shape) == tuple(weight.shape) else out[:, :weight.shape[1], :weight.shape[2]].contiguous()
 
 
-def _grad_bias(grad, groups: RowGroups) -> torch.Tensor:
+def _grad_bias(grad, groups: RowGroups, dtype: torch.dtype) -> torch.Tensor:
     outer = grad.shape[1]
     if groups.entries == 0:
-        return torch.zeros(groups.groups, outer, dtype=torch.bfloat16, device=grad.device)
+        return torch.zeros(groups.groups, outer, dtype=dtype, device=grad.device)
     dy = rows_of(grad)
-    out = torch.empty(groups.groups, outer, dtype=torch.bfloat16, device=grad.device)
+    out = torch.empty(groups.groups, outer, dtype=dtype, device=grad.device)
     _hip.launch("ep_hip_grouped_column_sums_bf16", grad.device,
-                dy.data_ptr(), dy.stride(0), groups.offsets.data_ptr(), groups.groups, outer, out.data_ptr(),
-                _hip.FLOAT_KINDS[torch.bfloat16])
+                dy.data_ptr(), dy.stride(0), groups.offsets.data_ptr(), groups.groups, outer, out.data_ptr(), _hip.FLOAT_KINDS[dtype])
     return out
 
 
@@ -110,7 +109,7 @@ class _GroupedLinear(torch.autograd.Function):
         need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
         return (_grad_rows(grad, weight, ctx.groups, ctx.x_grouped) if need_x else None,
                 _grad_weight(grad, x, weight, ctx.groups, ctx.x_grouped) if need_weight else None,
-                _grad_bias(grad, ctx.groups) if need_bias else None, None, None)
+                _grad_bias(grad, ctx.groups, torch.bfloat16) if need_bias else None, None, None)
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bias: torch.Tensor | None = None, *,
@@ -186,6 +185,7 @@ class _CompressedGrouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, biases, layer, groups, x_grouped):
         ctx.layer, ctx.groups, ctx.x_grouped = layer, groups, x_grouped
+        ctx.bias_dtype = biases.dtype if biases is not None and biases.dtype in _hip.FLOAT_KINDS else torch.float32      # of int8 experts, any
         return layer._product(x.detach(), biases, groups, x_grouped)
 
     @staticmethod
@@ -193,7 +193,7 @@ class _CompressedGrouped(torch.autograd.Function):
     def backward(ctx, grad):
         need_x, need_biases = ctx.needs_input_grad[:2]
         return (_grad_rows(grad, ctx.layer.dequantize(grad.device).to(grad.dtype), ctx.groups, ctx.x_grouped) if need_x else None,
-                _grad_bias(grad, ctx.groups) if need_biases else None, None, None, None)
+                _grad_bias(grad, ctx.groups, ctx.bias_dtype) if need_biases else None, None, None, None)
 
 
 class CompressedGroupedLinear(torch.nn.Module):

@@ -77,7 +77,7 @@ def test_a_gradient_with_a_tangent_is_refused(no_device, name, run, operands):
 @pytest.mark.parametrize("of_x", [False, True], ids=["biases alone", "and x"])
 def test_a_mixture_hands_its_biases_their_gradients(no_device, monkeypatch, of_x):
     monkeypatch.setattr(grouped, "_grad_rows", lambda grad, weight, plan, x_grouped: torch.full((3, 8), 2.0, dtype=grad.dtype))
-    monkeypatch.setattr(grouped, "_grad_bias", lambda grad, plan: torch.arange(20.0, dtype=grad.dtype).reshape(4, 5))
+    monkeypatch.setattr(grouped, "_grad_bias", lambda grad, plan, dtype: torch.arange(20.0, dtype=grad.dtype).reshape(4, 5))
     layer = ep.CompressedGroupedLinear([ep.CompressedLinear(8, 5) for _ in range(4)])
     layer._stacked = lambda device: _bf16(4, 5, 8)
     biases = [expert.bias.requires_grad_(True) for expert in layer.experts]
@@ -85,6 +85,18 @@ def test_a_mixture_hands_its_biases_their_gradients(no_device, monkeypatch, of_x
     layer(x, _plan()).sum().backward()
     assert torch.equal(torch.stack([bias.grad for bias in biases]), torch.arange(20.0).reshape(4, 5).bfloat16())
     assert (x.grad is not None) == of_x
+
+
+def test_biases_of_any_float_type_get_their_gradient(no_device, monkeypatch):
+    asked = []
+    monkeypatch.setattr(grouped, "_grad_bias", lambda grad, plan, dtype: asked.append(dtype) or torch.ones(4, 5, dtype=dtype))
+    monkeypatch.setattr(grouped.kernels, "quantize_rows", lambda rows: (torch.ones(rows.shape, dtype=torch.int8), torch.ones(len(rows))))
+    for dtype, sums in ((torch.float64, torch.float32), (torch.float32, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)):
+        layer = ep.CompressedGroupedLinear([ep.CompressedINT8Linear(16, 5) for _ in range(4)]).to(dtype)
+        layer._stacked = lambda device: torch.ones(4, 5, 16, dtype=torch.int8)
+        biases = [expert.bias.requires_grad_(True) for expert in layer.experts]
+        layer(_bf16(3, 16), _plan()).sum().backward()
+        assert asked.pop() == sums and all(bias.grad.dtype == dtype and bias.grad.eq(1).all() for bias in biases)
 
 
 @pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: torch.nn.Sequential(m).half()[0]], ids=["bf16", "half", "double", "inside a model"])

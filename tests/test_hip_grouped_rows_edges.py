@@ -117,6 +117,22 @@ def test_biases_of_compressed_experts_that_train_get_their_gradient(int8, of_x):
         assert torch.equal(layer(x, plan), frozen)
 
 
+def test_biases_in_f32_get_gradients_that_were_not_rounded_to_bf16():
+    """int8 experts of an f32 model keep f32 biases; the sums of the bf16 gradient's columns are f32."""
+    experts, outer, inner, tokens = 2, 40, 64, 300
+    torch.manual_seed(4)
+    layer = ep.CompressedGroupedLinear.from_linears([torch.nn.Linear(inner, outer) for _ in range(experts)], int8=True).cuda()
+    biases = [expert.bias.requires_grad_(True) for expert in layer.experts]
+    assert biases[0].dtype == torch.float32
+    plan = ep.group_rows(torch.arange(tokens, device="cuda") % experts, experts)
+    y = layer(torch.randn(tokens, inner, device="cuda").bfloat16(), plan)
+    dy = torch.randn(y.shape, device="cuda").bfloat16()
+    for g, grad in enumerate(torch.autograd.grad(y, biases, dy)):
+        rows = dy[int(plan.offsets[g]):int(plan.offsets[g + 1])].double()
+        assert grad.dtype == torch.float32
+        _within(grad, rows.sum(0), len(rows) * STEP_F32 * rows.abs().sum(0))
+
+
 def test_a_mixture_on_the_host_plans_once_and_one_that_leaves_the_device_lets_go():
     experts, outer, inner, tokens = 3, 72, 128, 40
     layer = ep.CompressedGroupedLinear.from_linears(_linears(experts, outer, inner), config=ep.EntroPackLossyConfig(target_bpp=4.0))
